@@ -241,6 +241,114 @@ typedef struct zmoe_combine_args {
 
 zmoe_status zmoe_combine(const zmoe_combine_args* a, zmoe_stream_t stream);
 
+/* --------------------------------------------------------------------------
+ * Gradients of the permute and the combine (no counterpart in the reference,
+ * which runs forward only): with them a router or adapters can be trained
+ * around expert rows that some other code differentiates.  Sums and dot
+ * products are fp32 in a fixed order, each output is rounded once; no atomics,
+ * so results repeat bit for bit.  H must be a multiple of 8, every row pointer
+ * 16-byte aligned.  row_of is zmoe_permute's; entries outside [0, rows) are
+ * slots without a row.
+ * ------------------------------------------------------------------------ */
+/* dx[t] = base[t] + sum_j dxp[row_of[t, j]] (no base term when NULL).  base may
+ * be dx itself. */
+typedef struct zmoe_permute_grad_args {
+  const uint16_t* dxp;        /* [rows, H] BF16 gradient of the gathered rows */
+  const int32_t* row_of;      /* [T, k] */
+  const uint16_t* base;       /* [T, H] BF16 gradient from other paths, or NULL */
+  int T, H, k, rows;
+  uint16_t* dx;               /* [T, H] BF16 out */
+} zmoe_permute_grad_args;
+
+zmoe_status zmoe_permute_grad(const zmoe_permute_grad_args* a, zmoe_stream_t stream);
+
+/* Gradient of zmoe_combine for the output gradient dout:
+ *   dy[row_of[t, j]] = w[t, j] dout[t]       dtopk_w[t, j] = <dout[t], y[row_of[t, j]]>
+ *   dy_shared[t] = g[t] dout[t]              dshared_gate[t] = <dout[t], y_shared[t]>
+ * mode SWITCH: a token without a row has dx[t] = w[t, 0] dout[t] and dtopk_w =
+ * <dout[t], x[t]>; dx[t] = 0 for the others.  Slots without a row otherwise
+ * have dtopk_w = 0.  Rows of dy that no slot names are left as they were. */
+typedef struct zmoe_combine_grad_args {
+  const uint16_t* dout;       /* [T, H] BF16 */
+  const uint16_t* y;          /* [rows, H] BF16 expert rows */
+  const uint16_t* y_shared;   /* [T, H] BF16 or NULL; read for dshared_gate */
+  const float* shared_gate;   /* [T] or NULL (a gate of 1) */
+  const int32_t* row_of;      /* [T, k] */
+  const float* topk_w;        /* [T, k] */
+  const uint16_t* x;          /* [T, H] BF16 (SWITCH) */
+  int T, H, k, mode, rows;
+  uint16_t* dy;               /* [rows, H] BF16 out */
+  float* dtopk_w;             /* [T, k] out */
+  uint16_t* dy_shared;        /* [T, H] BF16 out or NULL */
+  float* dshared_gate;        /* [T] out or NULL (needs y_shared) */
+  uint16_t* dx;               /* [T, H] BF16 out (SWITCH) */
+} zmoe_combine_grad_args;
+
+zmoe_status zmoe_combine_grad(const zmoe_combine_grad_args* a, zmoe_stream_t stream);
+
+/* --------------------------------------------------------------------------
+ * Low-rank adapters of many requests beside a shared projection (no
+ * counterpart in the reference: its experts stay compressed and are served
+ * as they are).  Adapter g holds A_g [R, H] and B_g [N, R]; a row of token t
+ * with adapter g gets
+ *   u = x[t] A_g^T          out[t] = base[t] + scale[g] * u B_g^T
+ * with base = the shared projection's output.  Rows are grouped by adapter:
+ * rows offsets[g] .. offsets[g + 1] belong to adapter g, row r is token
+ * token_of_row[r] (NULL: row r is token r, as for zmoe_permute's gathered
+ * rows with an adapter per expert).  Rows from offsets[G] to T use no adapter:
+ * out = base.  rank[g] <= R is the rank of adapter g: rows of A_g and columns
+ * of B_g from rank[g] on are not used, whatever they hold.
+ * ------------------------------------------------------------------------ */
+/* Rows of a batch from each token's adapter id: offsets [G + 1] and
+ * token_of_row [T], tokens ascending inside an adapter; ids outside [0, G) use
+ * no adapter and come last.  The plan serves every projection of a step. */
+zmoe_status zmoe_lora_plan(const int32_t* adapter, int T, int G, int32_t* offsets, int32_t* token_of_row,
+                           zmoe_stream_t stream);
+
+#define ZMOE_LORA_MAX_RANK 128
+
+typedef struct zmoe_lora_args {
+  const uint16_t* x;          /* [T, H] BF16 */
+  const uint16_t* base;       /* [T, N] BF16, NULL (zeros), or out itself */
+  const uint16_t* a;          /* [G, R, H] BF16 */
+  const uint16_t* b;          /* [G, N, R] BF16 */
+  const float* scale;         /* [G] or NULL (1) */
+  const int32_t* rank;        /* [G] or NULL (R); values are clamped to [0, R] */
+  const int32_t* offsets;     /* [G + 1] device */
+  const int32_t* token_of_row;/* [T] device or NULL */
+  int T, H, N, G, R;          /* H, N, R multiples of 8; R <= ZMOE_LORA_MAX_RANK */
+  uint16_t* out;              /* [T, N] BF16 */
+  float* u;                   /* [T, R] fp32 out by row, or NULL: x A^T, kept for zmoe_lora_grad; columns from
+                                 the rank on are 0, rows behind the last adapter's are left as they were */
+} zmoe_lora_args;
+
+zmoe_status zmoe_lora(const zmoe_lora_args* a, zmoe_stream_t stream);
+
+/* Gradient of zmoe_lora for the output gradient dy, with v = scale * dy B:
+ *   dx[t] = base[t] + v A      dA_g = sum of v^T x over the rows of g      dB_g = scale * sum of dy^T u
+ * (the gradient of zmoe_lora's base is dy itself).  Tokens without adapter:
+ * dx = base.  da and db are written whole: zeros for adapters without rows and
+ * from the rank on.  dx, or da and db, may be NULL. */
+typedef struct zmoe_lora_grad_args {
+  const uint16_t* dy;         /* [T, N] BF16 */
+  const uint16_t* x;          /* [T, H] BF16 */
+  const float* u;             /* [T, R] fp32 by row, zmoe_lora's */
+  const uint16_t* a;          /* [G, R, H] BF16 */
+  const uint16_t* b;          /* [G, N, R] BF16 */
+  const float* scale;         /* [G] or NULL (1) */
+  const int32_t* rank;        /* [G] or NULL (R) */
+  const int32_t* offsets;     /* [G + 1] device */
+  const int32_t* token_of_row;/* [T] device or NULL */
+  const uint16_t* base;       /* [T, H] BF16 gradient from other paths, NULL (zeros), or dx itself */
+  int T, H, N, G, R;
+  uint16_t* dx;               /* [T, H] BF16 out or NULL */
+  uint16_t* da;               /* [G, R, H] BF16 out or NULL */
+  uint16_t* db;               /* [G, N, R] BF16 out or NULL */
+  float* v;                   /* [T, R] fp32 scratch */
+} zmoe_lora_grad_args;
+
+zmoe_status zmoe_lora_grad(const zmoe_lora_grad_args* a, zmoe_stream_t stream);
+
 /* Row gather dst[r] = src[index[r]], r < rows, for rows of row_bytes bytes (a
  * multiple of 16; src and dst 16-byte aligned).  Regroups token rows received
  * from other ranks by expert, and back, under expert parallelism; the

@@ -20,6 +20,11 @@ zmoe_status launch_encode_chunks(const zmoe_enc_chunk*, int, int, uint32_t*, cud
 zmoe_status launch_router(const zmoe_router_args*, cudaStream_t);
 zmoe_status launch_permute(const zmoe_permute_args*, cudaStream_t);
 zmoe_status launch_combine(const zmoe_combine_args*, cudaStream_t);
+zmoe_status launch_permute_grad(const zmoe_permute_grad_args*, cudaStream_t);
+zmoe_status launch_combine_grad(const zmoe_combine_grad_args*, cudaStream_t);
+zmoe_status launch_lora_plan(const int32_t*, int, int, int32_t*, int32_t*, cudaStream_t);
+zmoe_status launch_lora(const zmoe_lora_args*, cudaStream_t);
+zmoe_status launch_lora_grad(const zmoe_lora_grad_args*, cudaStream_t);
 zmoe_status launch_gather_rows(const void*, const int32_t*, int, int, void*, cudaStream_t);
 
 }  // namespace zmoe
@@ -80,6 +85,27 @@ zmoe_status zmoe_gather_rows(const void* src, const int32_t* index, int rows, in
 
 zmoe_status zmoe_combine(const zmoe_combine_args* a, zmoe_stream_t stream) {
   return zmoe::launch_combine(a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+zmoe_status zmoe_permute_grad(const zmoe_permute_grad_args* a, zmoe_stream_t stream) {
+  return zmoe::launch_permute_grad(a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+zmoe_status zmoe_combine_grad(const zmoe_combine_grad_args* a, zmoe_stream_t stream) {
+  return zmoe::launch_combine_grad(a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+zmoe_status zmoe_lora_plan(const int32_t* adapter, int T, int G, int32_t* offsets, int32_t* token_of_row,
+                           zmoe_stream_t stream) {
+  return zmoe::launch_lora_plan(adapter, T, G, offsets, token_of_row, reinterpret_cast<cudaStream_t>(stream));
+}
+
+zmoe_status zmoe_lora(const zmoe_lora_args* a, zmoe_stream_t stream) {
+  return zmoe::launch_lora(a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+zmoe_status zmoe_lora_grad(const zmoe_lora_grad_args* a, zmoe_stream_t stream) {
+  return zmoe::launch_lora_grad(a, reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -7,6 +7,8 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <atomic>
+
 #include "../../include/zmoe.h"
 
 namespace zmoe {
@@ -42,6 +44,22 @@ inline zmoe_status launch_status(const char* what) {
 }
 
 constexpr int kNumSMs = 148;
+
+// Lets a kernel use all of an SM's shared memory (227 KB, of which up to 1 KB
+// static), once per device.  The same value is set whoever comes first, so concurrent first
+// calls agree.
+template <auto Kernel>
+zmoe_status allow_smem() {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  ZMOE_CUDA_RET(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(done.load(std::memory_order_relaxed) & bit)) {
+    ZMOE_CUDA_RET(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024));
+    done.fetch_or(bit, std::memory_order_relaxed);
+  }
+  return ZMOE_OK;
+}
 
 // Grouped expert FFN (ffn_tc.cu).  err: optional device word that a kernel
 // whose bounded wait ran out sets to 1.

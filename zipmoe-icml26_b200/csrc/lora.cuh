@@ -1,0 +1,71 @@
+// Shared by the adapter kernels: units of work from the row groups, and small helpers.
+#pragma once
+#include "common.cuh"
+
+namespace zmoe {
+namespace lora {
+
+constexpr int kThreads = 256;
+constexpr int kMaxCols = 32768;                        // H and N
+constexpr unsigned kFull = 0xffffffffu;
+
+// Up to `tile` consecutive rows of one group; g == G: the rows without adapter.
+struct Unit {
+  int g, row0, rows;                                   // rows == 0: no such unit
+};
+
+// Unit u of the groups' tiles, in order; `rest`: the rows behind the last
+// group are a group too.  Called by one full warp; offsets are clamped to
+// [0, T], so a unit never reaches past the last row.
+__device__ __forceinline__ Unit find_unit(const int32_t* __restrict__ offsets, int G, int T, int tile, bool rest, int u) {
+  const int lane = threadIdx.x & 31;
+  const int groups = G + (rest ? 1 : 0);
+  int before = 0;
+  for (int g0 = 0; g0 < groups; g0 += 32) {
+    const int g = g0 + lane;
+    int r0 = 0, n = 0;
+    if (g < groups) {
+      r0 = min(max(__ldg(offsets + g), 0), T);
+      const int r1 = g < G ? min(max(__ldg(offsets + g + 1), 0), T) : T;
+      n = max(0, r1 - r0);
+    }
+    const int tiles = (n + tile - 1) / tile;
+    int incl = tiles;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(kFull, incl, d);
+      if (lane >= d) incl += o;
+    }
+    const int first = before + incl - tiles;
+    const unsigned hit = __ballot_sync(kFull, u >= first && u < first + tiles);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const int local = u - __shfl_sync(kFull, first, src);
+      const int gr0 = __shfl_sync(kFull, r0, src), gn = __shfl_sync(kFull, n, src);
+      return Unit{g0 + src, gr0 + local * tile, min(tile, gn - local * tile)};
+    }
+    before += __shfl_sync(kFull, incl, 31);
+  }
+  return Unit{0, 0, 0};
+}
+
+// Token of a row, -1 when the list names none.
+__device__ __forceinline__ int token_of(const int32_t* token_of_row, int row, int T) {
+  const int t = token_of_row ? __ldg(token_of_row + row) : row;
+  return (unsigned)t < (unsigned)T ? t : -1;
+}
+
+// Columns of one of `parts` slices of n columns, in whole 16-byte vectors.
+__host__ __device__ __forceinline__ int slice8(int n, int parts) { return (n / 8 + parts - 1) / parts * 8; }
+
+__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    f[2 * q] = __uint_as_float(w[q] << 16);
+    f[2 * q + 1] = __uint_as_float(w[q] & 0xffff0000u);
+  }
+}
+
+}  // namespace lora
+}  // namespace zmoe

@@ -7,12 +7,33 @@
 // (csrc/dispatcher/expert_dispatcher.cpp:326-330).  The Switch capacity mask
 // is the cumsum over the sequence axis of the transformers<4.47 Top1 router.
 //
-// Three small launches: (1) one CTA per expert ranks its tokens in token order
-// with a block scan, drops those past the capacity of their sequence and writes
-// the count; (2) one CTA per expert turns counts into offsets and writes
-// row_of / token_of_row in the same order; (3) a grid-stride copy gathers the
-// activation rows with 16-byte accesses.
+// Without a capacity the order is a stable counting sort of the (token, slot)
+// pairs by expert.  Each warp of a cluster of CTAs takes a run of tokens, and
+// counts its experts in its own shared-memory row (lanes with the same expert
+// find each other with match.any, so a step of 32 pairs is one add per expert
+// present); prefixes over warps, CTAs (through distributed shared memory) and
+// experts turn the counts into first rows, and a second walk over the same
+// pairs hands the rows out in order.  No atomics: the result does not depend
+// on timing.  The activation rows are then copied token by token, so that x is
+// read once and each row is written once.
+//   * up to kFusedPairs pairs: one launch; every CTA sorts all pairs for
+//     itself and copies its own share of the rows, so that nothing waits on
+//     another CTA;
+//   * more: one cluster sorts, and the copy follows as a dependent launch that
+//     loads x while the sort finishes.
+//
+// With a capacity (Switch) drops depend on the rank within a sequence, and
+// three small launches do it: (1) one CTA per expert ranks its tokens in token
+// order with a block scan, drops those past the capacity of their sequence and
+// writes the count; (2) one CTA per expert turns counts into offsets and writes
+// row_of / token_of_row in the same order; (3) the copy.  They also take what
+// the sort's shared memory and steps do not hold (more than kSortE experts,
+// more than 32 slots).
+#include <cooperative_groups.h>
+
 #include "common.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace zmoe {
 namespace {
@@ -112,18 +133,205 @@ scatter_kernel(const int32_t* __restrict__ topk_idx, int T, int k, int E,
   }
 }
 
+// ---------------------------------------------------------------------------
+// counting sort
+// ---------------------------------------------------------------------------
+constexpr int kSortThreads = 1024;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortE = 1024;          // experts: one per thread in the scan, 128 KB of warp counts
+constexpr int kSortCluster = 8;
+constexpr int kFusedPairs = 2048;     // pairs every CTA of the fused launch sorts for itself
+constexpr int kBatch = 4;             // steps whose loads are issued together
+constexpr unsigned kFull = 0xffffffffu;
+
+struct SortArgs {
+  const int32_t* idx;                 // [T, k]
+  int T, k, E;
+  int rest;                           // 1: ids outside [0, E - 1) belong to the last group; 0: they have no row
+  int32_t* counts;                    // [E] or nullptr
+  int32_t* offsets;                   // [E + 1]; with rest the first E entries
+  int32_t* row_of;                    // [T, k] or nullptr
+  int32_t* token_of_row;              // [T * k]
+};
+
+// Sorts the pairs of tokens [0, T) by expert over the CTAs of a cluster (rank
+// of csize).  smem: hist [kSortWarps][E], tot [E], base [E], warp_sums.
+// write: this CTA writes the outputs in global memory.  rows_s (or nullptr)
+// receives every pair's row in shared memory.
+__device__ void sort_pairs(const SortArgs& a, int rank, int csize, int* smem, bool write, int32_t* rows_s) {
+  int* hist = smem;
+  int* tot = hist + kSortWarps * a.E;
+  int* base = tot + a.E;
+  int* warp_sums = base + a.E;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int k = a.k, E = a.E;
+  const int tp = 32 / k;                               // whole tokens per step of a warp
+  const int nw = kSortWarps * csize;
+  const int steps_all = (a.T + tp - 1) / tp;
+  const int per = (steps_all + nw - 1) / nw;           // steps per warp
+  const int s0 = min(steps_all, (rank * kSortWarps + warp) * per), s1 = min(steps_all, s0 + per);
+  const int jl = lane % k, tl = lane / k;              // slot and token of this lane in a step
+  const bool used = tl < tp;
+  const unsigned earlier = ((1u << lane) - 1u) & ~((1u << (lane - jl)) - 1u);   // same token, lower slots
+  int* my = hist + warp * E;
+
+  for (int e = lane; e < E; e += 32) my[e] = 0;
+  __syncwarp();
+
+  // one step: the expert of this lane's pair (-1: no row) and the lanes that share it
+  auto load = [&](int s) -> int {
+    const int t = s * tp + tl;
+    if (!used || s >= s1 || t >= a.T) return -2;
+    const int e = __ldg(a.idx + (size_t)t * k + jl);
+    if (a.rest) return (unsigned)e < (unsigned)(E - 1) ? e : E - 1;
+    return (unsigned)e < (unsigned)E ? e : -1;
+  };
+  auto peers = [&](int& e) -> unsigned {
+    unsigned m = __match_any_sync(kFull, e);
+    if (e >= 0 && (m & earlier)) e = -1;               // an expert named twice by a token counts once
+    return m & __ballot_sync(kFull, e >= 0);
+  };
+
+  for (int s = s0; s < s1; s += kBatch) {
+    int ev[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) ev[b] = load(s + b);
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      int e = ev[b];
+      const unsigned m = peers(e);
+      if (e >= 0 && lane == __ffs(m) - 1) my[e] += __popc(m);
+      __syncwarp();
+    }
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += kSortThreads) {
+    int run = 0;
+#pragma unroll 8
+    for (int w = 0; w < kSortWarps; ++w) {
+      const int n = hist[w * E + e];
+      hist[w * E + e] = run;
+      run += n;
+    }
+    tot[e] = run;
+  }
+  if (csize > 1) cg::this_cluster().sync();
+  else __syncthreads();
+  int all = 0, before = 0;
+  const int e1 = threadIdx.x;
+  if (e1 < E) {
+    if (csize > 1) {
+      for (int c = 0; c < csize; ++c) {
+        const int n = *cg::this_cluster().map_shared_rank(tot + e1, c);
+        if (c < rank) before += n;
+        all += n;
+      }
+    } else {
+      all = tot[e1];
+    }
+  }
+  int incl = all;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(kFull, incl, d);
+    if (lane >= d) incl += o;
+  }
+  if (lane == 31) warp_sums[warp] = incl;
+  __syncthreads();
+  if (warp == 0) {
+    int v = warp_sums[lane], si = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(kFull, si, d);
+      if (lane >= d) si += o;
+    }
+    warp_sums[lane] = si - v;
+  }
+  __syncthreads();
+  if (e1 < E) {
+    const int first = warp_sums[warp] + incl - all;
+    base[e1] = first + before;
+    if (write && rank == 0) {
+      if (a.counts) a.counts[e1] = all;
+      a.offsets[e1] = first;
+      if (e1 == E - 1 && !a.rest) a.offsets[E] = first + all;
+    }
+  }
+  __syncthreads();
+
+  for (int s = s0; s < s1; s += kBatch) {
+    int ev[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) ev[b] = load(s + b);
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      int e = ev[b];
+      const bool pair = e >= -1;
+      const unsigned m = peers(e);
+      const int t = (s + b) * tp + tl;
+      int row = -1;
+      if (e >= 0) row = base[e] + my[e] + __popc(m & ((1u << lane) - 1u));
+      __syncwarp();
+      if (e >= 0 && lane == __ffs(m) - 1) my[e] += __popc(m);
+      __syncwarp();
+      if (pair) {
+        if (rows_s) rows_s[t * k + jl] = row;
+        if (write) {
+          if (a.row_of) a.row_of[(size_t)t * k + jl] = row;
+          if (row >= 0) a.token_of_row[row] = t;
+        }
+      }
+    }
+  }
+}
+
+inline size_t sort_smem(int E) { return sizeof(int) * ((size_t)kSortWarps * E + 2 * (size_t)E + 32); }
+
+__global__ void __launch_bounds__(kSortThreads)
+sort_kernel(const SortArgs a) {
+  extern __shared__ int sort_smem_raw[];
+  cg::cluster_group cl = cg::this_cluster();
+  sort_pairs(a, (int)cl.block_rank(), (int)cl.num_blocks(), sort_smem_raw, true, nullptr);
+  // the last remote reads happened before the base scan's barriers of each
+  // CTA; wait for the cluster so that no CTA leaves while its totals are read
+  cl.sync();
+}
+
+// Every CTA sorts all pairs and copies the rows of its own share of the
+// 16-byte vectors; CTA 0 writes the index outputs.
+__global__ void __launch_bounds__(kSortThreads)
+sort_gather_kernel(const SortArgs a, const uint4* __restrict__ x, int vec, uint4* __restrict__ xp) {
+  extern __shared__ int sort_smem_raw[];
+  int32_t* rows_s = sort_smem_raw + kSortWarps * a.E + 2 * a.E + 32;
+  sort_pairs(a, 0, 1, sort_smem_raw, blockIdx.x == 0, rows_s);
+  __syncthreads();
+  const int total = a.T * vec;                         // the fused launch is small
+  for (int i = blockIdx.x * kSortThreads + threadIdx.x; i < total; i += gridDim.x * kSortThreads) {
+    const int t = i / vec, c = i - t * vec;
+    const uint4 v = __ldg(x + i);
+    for (int j = 0; j < a.k; ++j) {
+      const int r = rows_s[t * a.k + j];
+      if (r >= 0) xp[(size_t)r * vec + c] = v;
+    }
+  }
+}
+
+// xp[row_of[t, j]] = x[t] for every slot j with a row.  A dependent launch: x
+// was complete before the sort began, so its loads do not wait for the sort.
 __global__ void __launch_bounds__(kThreads)
-gather_kernel(const uint16_t* __restrict__ x, int H, const int32_t* __restrict__ offsets, int E,
-              const int32_t* __restrict__ token_of_row, uint16_t* __restrict__ xp, int max_rows) {
-  const int rows = min(offsets[E], max_rows);
-  const int vec = H / 8;
-  const size_t total = (size_t)rows * vec;
-  const size_t stride = (size_t)gridDim.x * blockDim.x;
-  for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += stride) {
-    const int r = (int)(i / vec);
-    const int c = (int)(i % vec);
-    const int t = token_of_row[r];
-    reinterpret_cast<uint4*>(xp + (size_t)r * H)[c] = __ldg(reinterpret_cast<const uint4*>(x + (size_t)t * H) + c);
+scatter_rows_kernel(const uint4* __restrict__ x, int T, int vec, int k, const int32_t* __restrict__ row_of,
+                    uint4* __restrict__ xp, int max_rows) {
+  const size_t first = (size_t)blockIdx.x * kThreads;
+  const unsigned rem = (unsigned)(first % vec) + threadIdx.x;
+  const size_t t = first / vec + rem / vec;
+  const unsigned c = rem % vec;
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (t < (size_t)T) v = __ldcs(x + t * vec + c);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (t >= (size_t)T) return;
+  for (int j = 0; j < k; ++j) {
+    const int r = row_of[t * k + j];
+    if ((unsigned)r < (unsigned)max_rows) __stcs(xp + (size_t)r * vec + c, v);
   }
 }
 
@@ -140,6 +348,28 @@ gather_rows_kernel(const uint4* __restrict__ src, const int32_t* __restrict__ in
   }
 }
 
+// One cluster: a single CTA while its 32 warps have at most four batches of
+// steps each, else the largest portable size.
+zmoe_status launch_sort(const SortArgs& a, cudaStream_t stream) {
+  const size_t smem = sort_smem(a.E);
+  zmoe_status st = allow_smem<sort_kernel>();
+  if (st != ZMOE_OK) return st;
+  const int tp = 32 / a.k, steps = (a.T + tp - 1) / tp;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(steps <= 4 * kBatch * kSortWarps ? 1 : kSortCluster);
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = cfg.gridDim.x;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  ZMOE_CUDA_RET(cudaLaunchKernelEx(&cfg, sort_kernel, a));
+  return launch_status("sort_kernel");
+}
+
 }  // namespace
 
 zmoe_status launch_permute(const zmoe_permute_args* a, cudaStream_t stream) {
@@ -150,26 +380,62 @@ zmoe_status launch_permute(const zmoe_permute_args* a, cudaStream_t stream) {
                  "permute: T=%d must be a multiple of seq_len=%d when capacity is set", a->T, a->seq_len);
   ZMOE_CHECK_ARG(a->xp == nullptr || (a->x && a->H % 8 == 0 && (uintptr_t)a->x % 16 == 0 && (uintptr_t)a->xp % 16 == 0),
                  "permute: gather needs H %% 8 == 0 and 16-byte aligned x/xp");
-  ZMOE_CUDA_RET(cudaMemsetAsync(a->row_of, 0xff, sizeof(int32_t) * (size_t)a->T * a->k, stream));
   if (a->T <= 0) {
     ZMOE_CUDA_RET(cudaMemsetAsync(a->counts, 0, sizeof(int32_t) * a->E, stream));
     ZMOE_CUDA_RET(cudaMemsetAsync(a->offsets, 0, sizeof(int32_t) * (a->E + 1), stream));
     return ZMOE_OK;
   }
-  count_kernel<<<a->E, kThreads, 0, stream>>>(a->topk_idx, a->T, a->k, a->capacity, a->seq_len, a->counts);
-  zmoe_status st = launch_status("count_kernel");
-  if (st != ZMOE_OK) return st;
-  scatter_kernel<<<a->E, kThreads, 0, stream>>>(a->topk_idx, a->T, a->k, a->E, a->counts, a->offsets,
-                                                a->row_of, a->token_of_row);
-  st = launch_status("scatter_kernel");
-  if (st != ZMOE_OK || a->xp == nullptr) return st;
-  const int max_rows = a->T * a->k;
-  size_t blocks = ((size_t)max_rows * (a->H / 8) + kThreads - 1) / kThreads;
-  if (blocks > (size_t)kNumSMs * 8) blocks = (size_t)kNumSMs * 8;
-  if (blocks == 0) blocks = 1;
-  gather_kernel<<<(unsigned)blocks, kThreads, 0, stream>>>(a->x, a->H, a->offsets, a->E, a->token_of_row,
-                                                            a->xp, max_rows);
-  return launch_status("gather_kernel");
+  ZMOE_CHECK_ARG((long long)a->T * a->k < (1LL << 31), "permute: T=%d x k=%d pairs are too many", a->T, a->k);
+  const int vec = a->H / 8;
+  zmoe_status st;
+  if (a->capacity <= 0 && a->E <= kSortE && a->k <= 32) {
+    const SortArgs sa{a->topk_idx, a->T, a->k, a->E, 0, a->counts, a->offsets, a->row_of, a->token_of_row};
+    if (a->xp && a->T * a->k <= kFusedPairs && vec > 0) {
+      st = allow_smem<sort_gather_kernel>();
+      if (st != ZMOE_OK) return st;
+      const size_t smem = sort_smem(a->E) + sizeof(int32_t) * (size_t)a->T * a->k;
+      int blocks = (int)(((size_t)a->T * vec + kSortThreads - 1) / kSortThreads);
+      if (blocks > kNumSMs) blocks = kNumSMs;
+      sort_gather_kernel<<<blocks, kSortThreads, smem, stream>>>(sa, reinterpret_cast<const uint4*>(a->x), vec,
+                                                                 reinterpret_cast<uint4*>(a->xp));
+      return launch_status("sort_gather_kernel");
+    }
+    st = launch_sort(sa, stream);
+  } else {
+    ZMOE_CUDA_RET(cudaMemsetAsync(a->row_of, 0xff, sizeof(int32_t) * (size_t)a->T * a->k, stream));
+    count_kernel<<<a->E, kThreads, 0, stream>>>(a->topk_idx, a->T, a->k, a->capacity, a->seq_len, a->counts);
+    st = launch_status("count_kernel");
+    if (st != ZMOE_OK) return st;
+    scatter_kernel<<<a->E, kThreads, 0, stream>>>(a->topk_idx, a->T, a->k, a->E, a->counts, a->offsets,
+                                                  a->row_of, a->token_of_row);
+    st = launch_status("scatter_kernel");
+  }
+  if (st != ZMOE_OK || a->xp == nullptr || vec == 0) return st;
+  const size_t blocks = ((size_t)a->T * vec + kThreads - 1) / kThreads;
+  ZMOE_CHECK_ARG(blocks < ((size_t)1 << 31), "permute: T=%d rows of H=%d are too many for one launch", a->T, a->H);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  ZMOE_CUDA_RET(cudaLaunchKernelEx(&cfg, scatter_rows_kernel, reinterpret_cast<const uint4*>(a->x), a->T, vec, a->k,
+                                   (const int32_t*)a->row_of, reinterpret_cast<uint4*>(a->xp), a->T * a->k));
+  return launch_status("scatter_rows_kernel");
+}
+
+zmoe_status launch_lora_plan(const int32_t* adapter, int T, int G, int32_t* offsets, int32_t* token_of_row,
+                             cudaStream_t stream) {
+  ZMOE_CHECK_ARG(G >= 1 && G < kSortE, "lora_plan: G=%d outside [1, %d]", G, kSortE - 1);
+  ZMOE_CHECK_ARG(T >= 0 && offsets && (T == 0 || (adapter && token_of_row)), "lora_plan: null pointer or negative T");
+  if (T == 0) {
+    ZMOE_CUDA_RET(cudaMemsetAsync(offsets, 0, sizeof(int32_t) * (size_t)(G + 1), stream));
+    return ZMOE_OK;
+  }
+  return launch_sort(SortArgs{adapter, T, 1, G + 1, 1, nullptr, offsets, nullptr, token_of_row}, stream);
 }
 
 zmoe_status launch_gather_rows(const void* src, const int32_t* index, int rows, int row_bytes, void* dst,

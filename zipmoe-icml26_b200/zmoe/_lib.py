@@ -57,6 +57,34 @@ class CombineArgs(ctypes.Structure):
                 ("mode", c_int), ("out", c_void_p)]
 
 
+class PermuteGradArgs(ctypes.Structure):
+    _fields_ = [("dxp", c_void_p), ("row_of", c_void_p), ("base", c_void_p), ("T", c_int), ("H", c_int),
+                ("k", c_int), ("rows", c_int), ("dx", c_void_p)]
+
+
+class CombineGradArgs(ctypes.Structure):
+    _fields_ = [("dout", c_void_p), ("y", c_void_p), ("y_shared", c_void_p), ("shared_gate", c_void_p),
+                ("row_of", c_void_p), ("topk_w", c_void_p), ("x", c_void_p), ("T", c_int), ("H", c_int),
+                ("k", c_int), ("mode", c_int), ("rows", c_int), ("dy", c_void_p), ("dtopk_w", c_void_p),
+                ("dy_shared", c_void_p), ("dshared_gate", c_void_p), ("dx", c_void_p)]
+
+
+class LoraArgs(ctypes.Structure):
+    _fields_ = [("x", c_void_p), ("base", c_void_p), ("a", c_void_p), ("b", c_void_p), ("scale", c_void_p),
+                ("rank", c_void_p), ("offsets", c_void_p), ("token_of_row", c_void_p), ("T", c_int), ("H", c_int),
+                ("N", c_int), ("G", c_int), ("R", c_int), ("out", c_void_p), ("u", c_void_p)]
+
+
+class LoraGradArgs(ctypes.Structure):
+    _fields_ = [("dy", c_void_p), ("x", c_void_p), ("u", c_void_p), ("a", c_void_p), ("b", c_void_p),
+                ("scale", c_void_p), ("rank", c_void_p), ("offsets", c_void_p), ("token_of_row", c_void_p),
+                ("base", c_void_p), ("T", c_int), ("H", c_int), ("N", c_int), ("G", c_int), ("R", c_int),
+                ("dx", c_void_p), ("da", c_void_p), ("db", c_void_p), ("v", c_void_p)]
+
+
+LORA_MAX_RANK = 128      # ZMOE_LORA_MAX_RANK
+
+
 class LayerConfig(ctypes.Structure):
     _fields_ = [("hidden", c_int), ("num_experts", c_int), ("inter", c_int), ("topk", c_int),
                 ("kind", c_int), ("route_mode", c_int), ("norm_topk_prob", c_int), ("scaling", c_float),
@@ -93,6 +121,11 @@ SIGNATURES = {
     "zmoe_expert_ffn": (c_int, [ctypes.POINTER(FfnArgs), c_void_p]),
     "zmoe_expert_ffn_noalloc": (c_int, [ctypes.POINTER(FfnArgs), c_void_p]),
     "zmoe_combine": (c_int, [ctypes.POINTER(CombineArgs), c_void_p]),
+    "zmoe_permute_grad": (c_int, [ctypes.POINTER(PermuteGradArgs), c_void_p]),
+    "zmoe_combine_grad": (c_int, [ctypes.POINTER(CombineGradArgs), c_void_p]),
+    "zmoe_lora_plan": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "zmoe_lora": (c_int, [ctypes.POINTER(LoraArgs), c_void_p]),
+    "zmoe_lora_grad": (c_int, [ctypes.POINTER(LoraGradArgs), c_void_p]),
     "zmoe_gather_rows": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p]),
     "zmoe_split_planes": (c_int, [c_void_p, ctypes.c_uint64, c_void_p, c_void_p]),
     "zmoe_lz4_compress_bound": (c_int, [c_int]),

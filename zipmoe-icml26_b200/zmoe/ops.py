@@ -12,7 +12,8 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import CombineArgs, FfnArgs, PermuteArgs, RouterArgs, ZmoeChunk, ZmoeEncChunk, check, lib
+from ._lib import (CombineArgs, CombineGradArgs, FfnArgs, LoraArgs, LoraGradArgs, PermuteArgs, PermuteGradArgs,
+                   RouterArgs, ZmoeChunk, ZmoeEncChunk, check, lib)
 
 ROUTE_QWEN, ROUTE_DEEPSEEK, ROUTE_SWITCH = 0, 1, 2
 
@@ -292,3 +293,151 @@ def combine(y: torch.Tensor, row_of: torch.Tensor, topk_w: torch.Tensor, mode: i
                     _ptr(x), T, H, k, mode, out.data_ptr())
     check(lib.zmoe_combine(ctypes.byref(a), _stream()), "zmoe_combine")
     return out
+
+
+# ---------------------------------------------------------------------------
+# gradients of permute and combine, low-rank adapters
+# ---------------------------------------------------------------------------
+_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
+
+
+def _arg(t: Optional[torch.Tensor], name: str, dtype, shape: tuple, device, optional: bool = False):
+    """Device pointer of an argument after checking its type, shape and place."""
+    if t is None:
+        if not optional:
+            raise ValueError(f"{name}: missing")
+        return None
+    if t.dtype != dtype or t.device != device or not t.is_contiguous() or tuple(t.shape) != shape:
+        raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {shape} on {device}, "
+                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _cuda(t: torch.Tensor, name: str, dims: int) -> torch.device:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != dims:
+        raise ValueError(f"{name}: expected a CUDA tensor with {dims} dimensions")
+    return t.device
+
+
+def _call(fn, args, device):
+    """Runs an entry point on the arguments' device and that device's current stream."""
+    if device.index == torch.cuda.current_device():
+        check(fn(ctypes.byref(args), _stream()), fn.__name__)
+    else:
+        with torch.cuda.device(device):
+            check(fn(ctypes.byref(args), _stream()), fn.__name__)
+
+
+def permute_grad(dxp: torch.Tensor, row_of: torch.Tensor, base: Optional[torch.Tensor] = None,
+                 dx: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of permute's gather (zmoe_permute_grad): dx[t] = base[t] + sum_j
+    dxp[row_of[t, j]].  base (the gradient from other paths) may be dx itself."""
+    dev = _cuda(dxp, "dxp", 2)
+    rows, H = dxp.shape
+    _cuda(row_of, "row_of", 2)
+    T, k = row_of.shape
+    if dx is None:
+        dx = torch.empty(T, H, dtype=_BF16, device=dev)
+    a = PermuteGradArgs(_arg(dxp, "dxp", _BF16, (rows, H), dev), _arg(row_of, "row_of", _I32, (T, k), dev),
+                        _arg(base, "base", _BF16, (T, H), dev, True), T, H, k, rows,
+                        _arg(dx, "dx", _BF16, (T, H), dev))
+    _call(lib.zmoe_permute_grad, a, dev)
+    return dx
+
+
+def combine_grad(dout: torch.Tensor, y: torch.Tensor, row_of: torch.Tensor, topk_w: torch.Tensor, mode: int,
+                 y_shared: Optional[torch.Tensor] = None, shared_gate: Optional[torch.Tensor] = None,
+                 x: Optional[torch.Tensor] = None, dy: Optional[torch.Tensor] = None):
+    """Gradient of combine (zmoe_combine_grad).  Returns dy, dtopk_w, dy_shared,
+    dshared_gate, dx; the last three are None without y_shared, without
+    shared_gate and outside Switch.  Rows of dy that no slot names are left as
+    they were (uninitialised when dy is not given)."""
+    dev = _cuda(dout, "dout", 2)
+    T, H = dout.shape
+    _cuda(y, "y", 2)
+    rows = y.shape[0]
+    _cuda(row_of, "row_of", 2)
+    k = row_of.shape[1]
+    if shared_gate is not None and y_shared is None:
+        raise ValueError("shared_gate without y_shared")
+    if dy is None:
+        dy = torch.empty(rows, H, dtype=_BF16, device=dev)
+    dw = torch.empty(T, k, dtype=_F32, device=dev)
+    dysh = torch.empty(T, H, dtype=_BF16, device=dev) if y_shared is not None else None
+    dg = torch.empty(T, dtype=_F32, device=dev) if shared_gate is not None else None
+    dx = torch.empty(T, H, dtype=_BF16, device=dev) if mode == ROUTE_SWITCH else None
+    a = CombineGradArgs(_arg(dout, "dout", _BF16, (T, H), dev), _arg(y, "y", _BF16, (rows, H), dev),
+                        _arg(y_shared, "y_shared", _BF16, (T, H), dev, True),
+                        _arg(shared_gate, "shared_gate", _F32, (T,), dev, True),
+                        _arg(row_of, "row_of", _I32, (T, k), dev), _arg(topk_w, "topk_w", _F32, (T, k), dev),
+                        _arg(x, "x", _BF16, (T, H), dev, mode != ROUTE_SWITCH), T, H, k, mode, rows,
+                        _arg(dy, "dy", _BF16, (rows, H), dev), dw.data_ptr(), _ptr(dysh), _ptr(dg), _ptr(dx))
+    _call(lib.zmoe_combine_grad, a, dev)
+    return dy, dw, dysh, dg, dx
+
+
+def lora_plan(adapter: torch.Tensor, G: int):
+    """Rows of a batch grouped by adapter (zmoe_lora_plan): adapter[t] in [0, G),
+    anything else for a token without one.  Returns offsets [G + 1] and
+    token_of_row [T], which serve every projection of the step."""
+    dev = _cuda(adapter, "adapter", 1)
+    T = adapter.shape[0]
+    offsets = torch.empty(max(G, 0) + 1, dtype=_I32, device=dev)
+    tor = torch.empty(T, dtype=_I32, device=dev)
+    ids = _arg(adapter, "adapter", _I32, (T,), dev)
+    with torch.cuda.device(dev):
+        check(lib.zmoe_lora_plan(ids, T, G, offsets.data_ptr(), tor.data_ptr(), _stream()), "zmoe_lora_plan")
+    return offsets, tor
+
+
+def _adapters(a: torch.Tensor, b: torch.Tensor, scale, rank, offsets, token_of_row, T: int, dev):
+    _cuda(a, "a", 3)
+    _cuda(b, "b", 3)
+    G, R, H = a.shape
+    N = b.shape[1]
+    return (G, R, H, N, _arg(a, "a", _BF16, (G, R, H), dev), _arg(b, "b", _BF16, (G, N, R), dev),
+            _arg(scale, "scale", _F32, (G,), dev, True), _arg(rank, "rank", _I32, (G,), dev, True),
+            _arg(offsets, "offsets", _I32, (G + 1,), dev), _arg(token_of_row, "token_of_row", _I32, (T,), dev, True))
+
+
+def lora(x: torch.Tensor, base: Optional[torch.Tensor], a: torch.Tensor, b: torch.Tensor,
+         scale: Optional[torch.Tensor], offsets: torch.Tensor, token_of_row: Optional[torch.Tensor] = None,
+         rank: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+         u: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Adapters of many requests beside a shared projection (zmoe_lora):
+    out[t] = base[t] + scale[g] (x[t] a[g]^T) b[g]^T for the rows of adapter g, out =
+    base for tokens without one.  a [G, R, H] and b [G, N, R] hold the adapters;
+    offsets and token_of_row come from lora_plan, or offsets from permute when
+    x holds its gathered rows (an adapter per expert).  out may be base; base
+    None counts as zeros.  u (fp32 [T, R]) receives x a^T for lora_grad."""
+    dev = _cuda(x, "x", 2)
+    T = x.shape[0]
+    G, R, H, N, pa, pb, ps, pr, po, pt = _adapters(a, b, scale, rank, offsets, token_of_row, T, dev)
+    if out is None:
+        out = torch.empty(T, N, dtype=_BF16, device=dev)
+    args = LoraArgs(_arg(x, "x", _BF16, (T, H), dev), _arg(base, "base", _BF16, (T, N), dev, True), pa, pb, ps, pr,
+                    po, pt, T, H, N, G, R, _arg(out, "out", _BF16, (T, N), dev), _arg(u, "u", _F32, (T, R), dev, True))
+    _call(lib.zmoe_lora, args, dev)
+    return out
+
+
+def lora_grad(dy: torch.Tensor, x: torch.Tensor, u: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
+              scale: Optional[torch.Tensor], offsets: torch.Tensor, token_of_row: Optional[torch.Tensor] = None,
+              rank: Optional[torch.Tensor] = None, base: Optional[torch.Tensor] = None,
+              dx: Optional[torch.Tensor] = None):
+    """Gradient of lora (zmoe_lora_grad) from its u: returns dx = base + v a, da and
+    db.  base (the gradient through the shared projection) may be dx itself;
+    the gradient of lora's own base is dy."""
+    dev = _cuda(dy, "dy", 2)
+    T = dy.shape[0]
+    G, R, H, N, pa, pb, ps, pr, po, pt = _adapters(a, b, scale, rank, offsets, token_of_row, T, dev)
+    if dx is None:
+        dx = torch.empty(T, H, dtype=_BF16, device=dev)
+    da, db = torch.empty_like(a), torch.empty_like(b)
+    v = torch.empty(T, R, dtype=_F32, device=dev)
+    args = LoraGradArgs(_arg(dy, "dy", _BF16, (T, N), dev), _arg(x, "x", _BF16, (T, H), dev),
+                        _arg(u, "u", _F32, (T, R), dev), pa, pb, ps, pr, po, pt,
+                        _arg(base, "base", _BF16, (T, H), dev, True), T, H, N, G, R,
+                        _arg(dx, "dx", _BF16, (T, H), dev), da.data_ptr(), db.data_ptr(), v.data_ptr())
+    _call(lib.zmoe_lora_grad, args, dev)
+    return dx, da, db
