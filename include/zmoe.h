@@ -54,8 +54,8 @@ zmoe_status zmoe_clock_probe(uint64_t* out, uint64_t window_ns, zmoe_stream_t st
 /* Human-readable text of the last error recorded on the calling thread. */
 const char* zmoe_last_error(void);
 
-/* Device-wide error word of the tcgen05 expert-FFN kernels on the current
- * device: 0, or 1 once a launch gave up one of its bounded mbarrier waits
+/* Device-wide error word of the tcgen05 expert-FFN and adapter kernels on the
+ * current device: 0, or 1 once a launch gave up one of its bounded mbarrier waits
  * (it then drained its own copies, freed its TMEM and returned, leaving its
  * outputs incomplete).  Synchronous; reset != 0 clears the word after reading.
  * No counterpart in the reference, whose libtorch FFN has no device waits. */

@@ -22,6 +22,7 @@ namespace {
 
 constexpr int kRows = 8;
 constexpr int kCluster = 8;
+constexpr int kRowsMaxT = 256;                         // longer batches go to the tensor cores
 constexpr int kRG = 4;                                 // rank rows per warp pass
 constexpr int kPre = 8;                                // 16-byte vectors of B loaded ahead of the sums
 
@@ -180,78 +181,6 @@ lora_rows_kernel(const zmoe_lora_args a) {
   cl.sync();                                           // partial sums stay until every CTA has read them
 }
 
-// ---------------------------------------------------------------------------
-// gradient
-// ---------------------------------------------------------------------------
-// Adapter of a row: the last g with offsets[g] <= row, or -1 behind the last.
-__device__ __forceinline__ int group_of(const int32_t* offsets, int G, int row) {
-  if (row >= offsets[G]) return -1;
-  int lo = 0, hi = G - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (offsets[mid] <= row) lo = mid; else hi = mid - 1;
-  }
-  return lo;
-}
-
-// v[row] = scale * dy[t] B, then dx[t] = base[t] + v A; one CTA per row.
-__global__ void __launch_bounds__(kThreads)
-lora_dx_kernel(const zmoe_lora_grad_args a) {
-  __shared__ float vs[ZMOE_LORA_MAX_RANK];
-  const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int t = token_of(a.token_of_row, row, a.T);
-  if (t < 0) return;
-  const int g = group_of(a.offsets, a.G, row);
-  const int rk = g < 0 ? 0 : (a.rank ? min(max(a.rank[g], 0), a.R) : a.R);
-  if (g >= 0) {
-    const float scale = a.scale ? a.scale[g] : 1.0f;
-    for (int r = warp; r < a.R; r += kThreads / 32) {
-      float s = 0.0f;
-      if (r < rk)
-        for (int n = lane; n < a.N; n += 32)
-          s = fmaf(bf16_bits_to_f32(a.dy[(size_t)t * a.N + n]), bf16_bits_to_f32(a.b[((size_t)g * a.N + n) * a.R + r]), s);
-#pragma unroll
-      for (int off = 16; off >= 1; off >>= 1) s += __shfl_xor_sync(kFull, s, off);
-      if (lane == 0) {
-        vs[r] = s * scale;
-        a.v[(size_t)row * a.R + r] = s * scale;
-      }
-    }
-  }
-  __syncthreads();
-  if (!a.dx || (g < 0 && a.dx == a.base)) return;
-  for (int h = threadIdx.x; h < a.H; h += kThreads) {
-    float s = 0.0f;
-    for (int r = 0; r < rk; ++r) s = fmaf(vs[r], bf16_bits_to_f32(a.a[((size_t)g * a.R + r) * a.H + h]), s);
-    if (a.base) s += bf16_bits_to_f32(a.base[(size_t)t * a.H + h]);
-    a.dx[(size_t)t * a.H + h] = f32_to_bf16_bits(s);
-  }
-}
-
-// dA (out [R, M], src = x, f = v) and dB (out [M, R], src = dy, f = u, scaled):
-// one thread per column m of src, for one rank index r and adapter g.
-__global__ void __launch_bounds__(kThreads)
-lora_dw_kernel(const zmoe_lora_grad_args a, int which) {
-  const int M = which ? a.N : a.H, m = blockIdx.x * kThreads + threadIdx.x, r = blockIdx.y, g = blockIdx.z;
-  if (m >= M) return;
-  const int rk = a.rank ? min(max(a.rank[g], 0), a.R) : a.R;
-  const int r0 = min(max(a.offsets[g], 0), a.T), r1 = min(max(a.offsets[g + 1], 0), a.T);
-  const uint16_t* src = which ? a.dy : a.x;
-  const float* f = which ? a.u : a.v;
-  float s = 0.0f;
-  if (r < rk)
-    for (int row = r0; row < r1; ++row) {
-      const int t = token_of(a.token_of_row, row, a.T);
-      if (t >= 0) s = fmaf(f[(size_t)row * a.R + r], bf16_bits_to_f32(src[(size_t)t * M + m]), s);
-    }
-  if (which) {
-    if (a.scale) s *= a.scale[g];
-    a.db[((size_t)g * M + m) * a.R + r] = f32_to_bf16_bits(s);
-  } else {
-    a.da[((size_t)g * a.R + r) * M + m] = f32_to_bf16_bits(s);
-  }
-}
-
 bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
 
 }  // namespace
@@ -269,10 +198,10 @@ zmoe_status launch_lora(const zmoe_lora_args* a, cudaStream_t stream) {
   ZMOE_CHECK_ARG(aligned16(a->x) && aligned16(a->base) && aligned16(a->a) && aligned16(a->b) && aligned16(a->out) &&
                      aligned16(a->u), "lora: rows must be 16-byte aligned");
   ZMOE_CHECK_ARG(a->H <= kMaxCols && a->N <= kMaxCols, "lora: H=%d or N=%d above %d", a->H, a->N, kMaxCols);
+  if (a->T > kRowsMaxT) return launch_tiles(a, stream);
   zmoe_status st = allow_smem<lora_rows_kernel>();
   if (st != ZMOE_OK) return st;
   const size_t units = (size_t)a->T / kRows + (size_t)(a->T < a->G + 1 ? a->T : a->G + 1);
-  ZMOE_CHECK_ARG(units * kCluster < ((size_t)1 << 31), "lora: T=%d rows are too many for one launch", a->T);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(units * kCluster));
   cfg.blockDim = dim3(kThreads);
@@ -310,16 +239,7 @@ zmoe_status launch_lora_grad(const zmoe_lora_grad_args* a, cudaStream_t stream) 
   ZMOE_CHECK_ARG(aligned16(a->dy) && aligned16(a->x) && aligned16(a->u) && aligned16(a->a) && aligned16(a->b) &&
                      aligned16(a->base) && aligned16(a->dx) && aligned16(a->da) && aligned16(a->db) && aligned16(a->v),
                  "lora_grad: rows must be 16-byte aligned");
-  lora_dx_kernel<<<a->T, kThreads, 0, stream>>>(*a);
-  zmoe_status st = launch_status("lora_dx_kernel");
-  if (st != ZMOE_OK || !a->da) return st;
-  for (int which = 0; which < 2; ++which) {
-    const int M = which ? a->N : a->H;
-    lora_dw_kernel<<<dim3((M + kThreads - 1) / kThreads, a->R, a->G), kThreads, 0, stream>>>(*a, which);
-    st = launch_status("lora_dw_kernel");
-    if (st != ZMOE_OK) return st;
-  }
-  return ZMOE_OK;
+  return launch_grad_tiles(a, stream);
 }
 
 }  // namespace zmoe

@@ -9,6 +9,11 @@ constexpr int kThreads = 256;
 constexpr int kMaxCols = 32768;                        // H and N
 constexpr unsigned kFull = 0xffffffffu;
 
+// lora_tc.cu
+zmoe_status launch_tiles(const zmoe_lora_args* a, cudaStream_t stream);
+zmoe_status launch_grad_tiles(const zmoe_lora_grad_args* a, cudaStream_t stream);
+zmoe_status read_error(int32_t* out, int reset);
+
 // Up to `tile` consecutive rows of one group; g == G: the rows without adapter.
 struct Unit {
   int g, row0, rows;                                   // rows == 0: no such unit
