@@ -320,6 +320,7 @@ typedef struct zmoe_lora_args {
   uint16_t* out;              /* [T, N] BF16 */
   float* u;                   /* [T, R] fp32 out by row, or NULL: x A^T, kept for zmoe_lora_grad; columns from
                                  the rank on are 0, rows behind the last adapter's are left as they were */
+  float* scratch;             /* [T, R] fp32 */
 } zmoe_lora_args;
 
 zmoe_status zmoe_lora(const zmoe_lora_args* a, zmoe_stream_t stream);
@@ -344,7 +345,7 @@ typedef struct zmoe_lora_grad_args {
   uint16_t* dx;               /* [T, H] BF16 out or NULL */
   uint16_t* da;               /* [G, R, H] BF16 out or NULL */
   uint16_t* db;               /* [G, N, R] BF16 out or NULL */
-  float* v;                   /* [T, R] fp32 scratch */
+  float* scratch;             /* [T, 2 R] fp32 */
 } zmoe_lora_grad_args;
 
 zmoe_status zmoe_lora_grad(const zmoe_lora_grad_args* a, zmoe_stream_t stream);

@@ -56,15 +56,15 @@ def test_combine_grad_refuses():
 
 def test_lora_refuses():
     L = _lib()
-    ok = dict(x=P, base=P, a=P, b=P, scale=P, rank=None, offsets=P, token_of_row=None, T=4, H=16, N=16, G=2, R=8, out=P)
+    ok = dict(x=P, base=P, a=P, b=P, scale=P, rank=None, offsets=P, token_of_row=None, T=4, H=16, N=16, G=2, R=8, out=P, scratch=P)
     for kw, text in (({"R": 12}, b"R=12"), ({"R": 136}, b"R=136"), ({"R": 0}, b"R=0"), ({"H": 20}, b"H=20"),
                      ({"N": 4}, b"N=4"), ({"G": 0}, b"G < 1"), ({"T": -1}, b"T < 0"), ({"x": None}, b"null"),
-                     ({"offsets": None}, b"null"), ({"a": P + 2}, b"aligned"), ({"out": P + 8}, b"aligned"),
+                     ({"offsets": None}, b"null"), ({"scratch": None}, b"null"), ({"a": P + 2}, b"aligned"), ({"out": P + 8}, b"aligned"),
                      ({"H": 32776}, b"above")):
         _refused(L.lib.zmoe_lora, L.LoraArgs(**dict(ok, **kw)), text)
     ok = dict(dy=P, x=P, u=P, a=P, b=P, scale=P, rank=None, offsets=P, token_of_row=None, base=None, T=4, H=16, N=16,
-              G=2, R=8, dx=P, da=P, db=P, v=P)
-    for kw, text in (({"da": None}, b"together"), ({"dx": None, "da": None, "db": None}, b"no output"), ({"v": None}, b"null"),
+              G=2, R=8, dx=P, da=P, db=P, scratch=P)
+    for kw, text in (({"da": None}, b"together"), ({"dx": None, "da": None, "db": None}, b"no output"), ({"scratch": None}, b"null"),
                      ({"u": None}, b"null"), ({"R": 12}, b"R=12"), ({"dy": P + 2}, b"aligned"), ({"G": 0}, b"G < 1")):
         _refused(L.lib.zmoe_lora_grad, L.LoraGradArgs(**dict(ok, **kw)), text)
     assert L.lib.zmoe_lora_plan(P, 4, 0, P, P, None) == 1

@@ -194,9 +194,9 @@ zmoe_status launch_lora(const zmoe_lora_args* a, cudaStream_t stream) {
   ZMOE_CHECK_ARG(a->R > 0 && a->R % 8 == 0 && a->R <= ZMOE_LORA_MAX_RANK, "lora: R=%d must be a multiple of 8 in [8, %d]",
                  a->R, ZMOE_LORA_MAX_RANK);
   if (a->T == 0) return ZMOE_OK;
-  ZMOE_CHECK_ARG(a->x && a->a && a->b && a->offsets && a->out, "lora: null pointer");
+  ZMOE_CHECK_ARG(a->x && a->a && a->b && a->offsets && a->out && a->scratch, "lora: null pointer");
   ZMOE_CHECK_ARG(aligned16(a->x) && aligned16(a->base) && aligned16(a->a) && aligned16(a->b) && aligned16(a->out) &&
-                     aligned16(a->u), "lora: rows must be 16-byte aligned");
+                     aligned16(a->u) && aligned16(a->scratch), "lora: rows must be 16-byte aligned");
   ZMOE_CHECK_ARG(a->H <= kMaxCols && a->N <= kMaxCols, "lora: H=%d or N=%d above %d", a->H, a->N, kMaxCols);
   if (a->T > kRowsMaxT) return launch_tiles(a, stream);
   zmoe_status st = allow_smem<lora_rows_kernel>();
@@ -235,9 +235,9 @@ zmoe_status launch_lora_grad(const zmoe_lora_grad_args* a, cudaStream_t stream) 
     }
     return ZMOE_OK;
   }
-  ZMOE_CHECK_ARG(a->dy && a->a && a->b && a->offsets && a->v && (!a->da || (a->x && a->u)), "lora_grad: null pointer");
+  ZMOE_CHECK_ARG(a->dy && a->a && a->b && a->offsets && a->scratch && (!a->da || (a->x && a->u)), "lora_grad: null pointer");
   ZMOE_CHECK_ARG(aligned16(a->dy) && aligned16(a->x) && aligned16(a->u) && aligned16(a->a) && aligned16(a->b) &&
-                     aligned16(a->base) && aligned16(a->dx) && aligned16(a->da) && aligned16(a->db) && aligned16(a->v),
+                     aligned16(a->base) && aligned16(a->dx) && aligned16(a->da) && aligned16(a->db) && aligned16(a->scratch),
                  "lora_grad: rows must be 16-byte aligned");
   return launch_grad_tiles(a, stream);
 }

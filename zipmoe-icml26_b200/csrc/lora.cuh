@@ -8,6 +8,7 @@ namespace lora {
 constexpr int kThreads = 256;
 constexpr int kMaxCols = 32768;                        // H and N
 constexpr unsigned kFull = 0xffffffffu;
+constexpr int kAhead = 4;                              // of find_unit
 
 // lora_tc.cu
 zmoe_status launch_tiles(const zmoe_lora_args* a, cudaStream_t stream);
@@ -26,30 +27,38 @@ __device__ __forceinline__ Unit find_unit(const int32_t* __restrict__ offsets, i
   const int lane = threadIdx.x & 31;
   const int groups = G + (rest ? 1 : 0);
   int before = 0;
-  for (int g0 = 0; g0 < groups; g0 += 32) {
-    const int g = g0 + lane;
-    int r0 = 0, n = 0;
-    if (g < groups) {
-      r0 = min(max(__ldg(offsets + g), 0), T);
-      const int r1 = g < G ? min(max(__ldg(offsets + g + 1), 0), T) : T;
-      n = max(0, r1 - r0);
-    }
-    const int tiles = (n + tile - 1) / tile;
-    int incl = tiles;
+  for (int g0 = 0; g0 < groups; g0 += 32 * kAhead) {
+    int r0[kAhead], n[kAhead];                         // kAhead warps of groups, loaded together
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int o = __shfl_up_sync(kFull, incl, d);
-      if (lane >= d) incl += o;
+    for (int i = 0; i < kAhead; ++i) {
+      const int g = g0 + 32 * i + lane;
+      r0[i] = n[i] = 0;
+      if (g < groups) {
+        r0[i] = min(max(__ldg(offsets + g), 0), T);
+        const int r1 = g < G ? min(max(__ldg(offsets + g + 1), 0), T) : T;
+        n[i] = max(0, r1 - r0[i]);
+      }
     }
-    const int first = before + incl - tiles;
-    const unsigned hit = __ballot_sync(kFull, u >= first && u < first + tiles);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      const int local = u - __shfl_sync(kFull, first, src);
-      const int gr0 = __shfl_sync(kFull, r0, src), gn = __shfl_sync(kFull, n, src);
-      return Unit{g0 + src, gr0 + local * tile, min(tile, gn - local * tile)};
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int tiles = (n[i] + tile - 1) / tile;
+      int incl = tiles;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(kFull, incl, d);
+        if (lane >= d) incl += o;
+      }
+      const int first = before + incl - tiles;
+      const unsigned hit = __ballot_sync(kFull, u >= first && u < first + tiles);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        const int local = u - __shfl_sync(kFull, first, src);
+        const int gr0 = __shfl_sync(kFull, r0[i], src), gn = __shfl_sync(kFull, n[i], src);
+        return Unit{g0 + 32 * i + src, gr0 + local * tile, min(tile, gn - local * tile)};
+      }
+      before += __shfl_sync(kFull, incl, 31);
+      if (g0 + 32 * (i + 1) >= groups) break;
     }
-    before += __shfl_sync(kFull, incl, 31);
   }
   return Unit{0, 0, 0};
 }

@@ -1,16 +1,22 @@
 // Low-rank adapters on the 5th-generation tensor cores (tcgen05 + TMEM).
 //
-// lora_tile_kernel: two chained products for a tile of 128 rows of one adapter,
-//   DIR 0, forward:   u = x A^T [128, R]       out = base + (s u) B^T
-//   DIR 1, gradient:  v = s dy B [128, R]      dx  = base + v A
-// by a thread-block cluster of C CTAs.  CTA c sums a slice of the long first
-// contraction (H or N); the partial [128, R] sums meet in fp32 through
-// distributed shared memory, and CTA c computes a slice of the output columns.
-// The work is bound by HBM: rows in, base in, rows out, each once.
-//
-// lora_dw_kernel: dA^T [H, R] = x^T v and dB [N, R] = s dy^T u, the rows of the
-// adapter as the contraction, one tile of 128 columns of x or dy per cluster,
-// whose CTAs share the rows; partial sums meet the same way, in rank order.
+// Three kernels, each bound by HBM (their MMAs are narrow):
+//   lora_shrink_kernel  u = x A^T (forward) or v = s dy B (gradient) for tiles of
+//                       128 rows of one adapter.  A cluster of C CTAs splits the
+//                       long contraction (H or N) of a tile; the partial
+//                       [128, R] sums meet in fp32 through distributed shared
+//                       memory, each CTA adding its share of the columns in rank
+//                       order.
+//   lora_expand_kernel  out = base + s u B^T or dx = base + v A: a CTA per (tile,
+//                       share of the output columns).  Launched as a dependent of
+//                       the shrink: it loads base and weights while that ends.
+//   lora_dw_kernel      dA^T = x^T v and dB = s dy^T u: the rows of an adapter as
+//                       the contraction, one tile of 128 columns of x or dy per
+//                       cluster, whose CTAs share the rows.
+// (A single kernel for shrink and expand, with u kept in TMEM, measured slower:
+// 31.5 against 29 us for 8191 rows of 2048 in and out at rank 64, 40 against 20 us
+// for 2047 rows of 2048 in and 5632 out at rank 16: tiles of whole rows leave SMs
+// without work.)
 //
 // Precision: x, dy, A and B are BF16 as given.  u and v are fp32 sums; as
 // operands of the second product they are carried as two BF16 values each
@@ -18,16 +24,18 @@
 // second product costs twice the MMAs, which HBM hides, and the output has one
 // visible rounding.
 //
-// Operands come in by cp.async (rows are gathered by token, 16 bytes a lane)
-// into 128-byte-swizzled tiles, kStages deep.  Every column beyond an
-// adapter's rank, every row beyond a tile and every column beyond a matrix is
-// filled with zeros there, whatever memory holds.  One thread issues the MMAs;
-// all threads load and drain, one __syncthreads per step.  Two CTAs fit an SM
-// (R <= 64), so that one loads while the other drains.
+// Warps have roles: some load, one issues the MMAs, some drain TMEM.  Operands
+// come in by cp.async (rows are gathered by token, 16 bytes a lane) into
+// 128-byte-swizzled tiles of a ring, whose slots pass from role to role by
+// mbarriers, so that no step waits for the whole CTA.  Every column beyond an
+// adapter's rank and every column beyond a matrix is filled with zeros there,
+// whatever memory holds.  Two CTAs fit an SM (R <= 64).
 //
-// Waits for MMAs are bounded: on a timeout the CTA sets the device error word
-// (zmoe_kernel_error), stops waiting and runs through to its end, so that no
-// CTA of its cluster is left at a barrier; its outputs are then incomplete.
+// Every mbarrier wait is bounded: on a timeout the CTA sets the device error
+// word (zmoe_kernel_error), stops waiting and runs through to its end, so that
+// no CTA of its cluster is left at a barrier; its outputs are then incomplete.
+// TMEM allocations wait for nothing but CTAs that end by themselves: shared
+// memory admits no more CTAs of these kernels to an SM than its 512 columns hold.
 #include <cooperative_groups.h>
 
 #include "lora.cuh"
@@ -46,9 +54,7 @@ using namespace tc;
 
 constexpr int kTile = 128;                             // rows per tile (MMA M)
 constexpr int kStep = 64;                              // contraction or output columns per step: 128 bytes
-constexpr int kStages = 3;
 constexpr int kXBytes = kTile * kStep * 2;             // 16 KB
-constexpr uint32_t kTmemCols = 256;                    // [0, 128): first product, [128, 256): two 64-column outputs
 constexpr long long kWaitLimit = 4000000000LL;         // about 2 s at 1.9 GHz
 
 // fp32 D, BF16 A and B, M = 128; amn / bmn: the operand's M or N index is contiguous
@@ -69,10 +75,40 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t block) {
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// One arrival on bar once this thread's copies so far have landed.  The copies
+// are ordinary writes to the tensor cores' asynchronous reads, so the MMA warp
+// fences between its wait and its MMAs.
+__device__ __forceinline__ void cp_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// The MMA warp runs its loop with all lanes, so that barrier addresses and
+// descriptors stay in uniform registers; `go` is true in the one lane that issues.
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                       uint32_t accumulate, uint32_t go) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(go)
+      : "memory");
+}
+
+// One lane of a converged warp.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t go;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(go));
+  return go;
+}
 
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&f)[8]) {
   uint32_t r[8];
@@ -84,19 +120,59 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&f)[8]) {
   for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(r[i]);
 }
 
-// Bounded; after the first timeout the CTA no longer waits.
-__device__ __forceinline__ void wait_bar(uint64_t* bar, uint32_t parity, volatile int* failed) {
-  if (!mbar_try_wait(bar, parity)) {
-    const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity)) {
-      if (*failed) break;
-      if (clock64() - t0 > kWaitLimit) {
-        *failed = 1;
-        atomicExch(&g_lora_error, 1);
-        break;
-      }
+// 32 columns, 16 at a time, one wait.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&lo)[16], uint32_t (&hi)[16]) {
+  tmem_ld16(taddr, lo);
+  tmem_ld16(taddr + 16, hi);
+  tmem_wait_ld();
+}
+
+__device__ __forceinline__ bool try_wait_at(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ void commit_at(uint32_t bar, uint32_t go) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(go)
+      : "memory");
+}
+
+// Place of a step in the ring: slot, and the parity of the slot's use.
+template <int N>
+struct Ring {
+  uint32_t slot = 0, parity = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == N) {
+      slot = 0;
+      parity ^= 1u;
     }
   }
+};
+
+// Bounded wait of one thread; after the first timeout the CTA no longer waits.
+__device__ __forceinline__ void wait_one(uint32_t bar, uint32_t parity, volatile int* failed) {
+  if (try_wait_at(bar, parity)) return;
+  const long long t0 = clock64();
+  while (!try_wait_at(bar, parity)) {
+    if (*failed) return;
+    if (clock64() - t0 > kWaitLimit) {
+      *failed = 1;
+      atomicExch(&g_lora_error, 1);
+      return;
+    }
+  }
+}
+__device__ __forceinline__ void wait_bar(uint32_t bar, uint32_t parity, volatile int* failed) {
+  wait_one(bar, parity, failed);
   __syncwarp();
 }
 
@@ -106,7 +182,8 @@ __device__ __forceinline__ uint32_t place(int row, int chunk, uint32_t block) {
 }
 
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
-  return (uint32_t)f32_to_bf16_bits(a) | ((uint32_t)f32_to_bf16_bits(b) << 16);
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 // Eight fp32 values as two BF16 vectors, f = hi + lo up to 2^-16; an infinite
@@ -115,108 +192,173 @@ __device__ __forceinline__ void split8(const float (&f)[8], uint4& hi, uint4& lo
   uint32_t h[4], l[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    float r[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float v = f[2 * q + i], b = round_bf16(v);
-      r[i] = fabsf(b) <= 3.4e38f ? v - b : 0.0f;
-    }
     h[q] = pack2(f[2 * q], f[2 * q + 1]);
-    l[q] = pack2(r[0], r[1]);
+    const float b0 = __uint_as_float(h[q] << 16), b1 = __uint_as_float(h[q] & 0xffff0000u);
+    l[q] = pack2(fabsf(b0) <= 3.4e38f ? f[2 * q] - b0 : 0.0f, fabsf(b1) <= 3.4e38f ? f[2 * q + 1] - b1 : 0.0f);
   }
   hi = make_uint4(h[0], h[1], h[2], h[3]);
   lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
 struct TileArgs {
-  const uint16_t* src;                                 // [T, K1] rows of the first product
+  const uint16_t* src;                                 // shrink: [T, K1]
   const uint16_t* w1;                                  // DIR 0: A [G, R, K1]; DIR 1: B [G, K1, R]
   const uint16_t* w2;                                  // DIR 0: B [G, K2, R]; DIR 1: A [G, R, K2]
-  const uint16_t* base;                                // [T, K2] or nullptr
+  const uint16_t* base;                                // expand: [T, K2] or nullptr
   const float* scale;
   const int32_t *rank, *offsets, *token_of_row;
   int T, K1, K2, G, R;
-  uint16_t* out;                                       // [T, K2] or nullptr (DIR 1: only v)
-  float* u;                                            // [T, R] or nullptr: u (DIR 0) or s dy B (DIR 1)
+  uint16_t* out;                                       // [T, K2]
+  float* u;                                            // DIR 0: [T, R] out or nullptr
+  const float* u_in;                                   // DIR 1: the forward pass's u, [T, R], or nullptr
+  uint16_t* split;                                     // DIR 0: [T][s u hi, lo][R]; DIR 1: [T][v hi, lo, u hi, lo][R]
+  int parts;                                           // expand: CTAs per tile
 };
 
 __device__ __forceinline__ int rank_of(const int32_t* rank, int g, int R) {
-  return rank ? min(max(rank[g], 0), R) : R;
+  return rank ? min(max(__ldg(rank + g), 0), R) : R;
 }
 
+constexpr int kLoadWarps = 4, kLoaders = 32 * kLoadWarps;
+
+// The places and sources of a loader thread's pieces of the weights, fixed but
+// for a step's constant move: rows of the rank x 64 columns (A), or 64 rows x
+// columns of the rank (B).
+template <int RB, bool RANK_ROWS>
+struct Weights {
+  uint32_t at[RB * 4];                                 // place << 5 | bytes; 31: no piece
+  int off[RB * 4];                                     // B: row * R + 8 chunk
+  const uint16_t* p;
+  const uint16_t* any;                                 // a valid address for pieces of no bytes
+  size_t row16;                                        // A: 16 rows
+  int left, col, K, R, rk, rp, lt;
+
+  __device__ __forceinline__ Weights(const uint16_t* w, int g, int K_, int R_, int rk_, int rp_, int lt_, int step0)
+      : any(w), K(K_), R(R_), rk(rk_), rp(rp_), lt(lt_) {
+    col = step0 * kStep + 8 * (lt & 7);
+    row16 = (size_t)16 * K;
+    left = (K - step0 * kStep) * R;
+    if (RANK_ROWS) {
+      p = w + ((size_t)g * R + (lt >> 3)) * K + col;
+    } else {
+      p = w + ((size_t)g * K + step0 * kStep) * R;
+      const int n8 = rp / 8;
+      const uint32_t inv = (65536u + n8 - 1) / n8;     // exact for the indexes below 64 n8 <= 1024
+#pragma unroll
+      for (int i = 0; i < RB * 4; ++i) {
+        const int it = lt + i * kLoaders, n = (int)((it * inv) >> 16), c = it - n * n8;
+        at[i] = n < kStep ? place(n, c, 8192) << 5 | (uint32_t)min(max(2 * (rk - 8 * c), 0), 16) : 31u;
+        off[i] = n * R + 8 * c;
+      }
+    }
+  }
+  // The pieces of this step into dst (and xo: place of row lt / 8, chunk lt % 8), then `steps` on.
+  __device__ __forceinline__ void load(uint32_t dst, uint32_t xo, int steps) {
+    if (RANK_ROWS) {
+#pragma unroll
+      for (int e = 0; e < RB * 4; ++e) {
+        const int r = (lt >> 3) + 16 * e;
+        if (r < rp) {
+          const bool in = r < rk && col < K;
+          cp16(dst + xo + 2048u * e, in ? p + e * row16 : any, in ? 16 : 0);
+        }
+      }
+      p += steps * kStep;
+      col += steps * kStep;
+    } else {
+#pragma unroll
+      for (int e = 0; e < RB * 4; ++e) {
+        if (at[e] != 31u) {
+          const int bytes = off[e] < left ? (int)(at[e] & 31u) : 0;
+          cp16(dst + (at[e] >> 5), bytes ? p + off[e] : any, bytes);
+        }
+      }
+      p += (size_t)(steps * kStep) * R;
+      left -= steps * kStep * R;
+    }
+  }
+};
+
+// Eight rows of a 128 x 64 tile of x or base: rows lt / 8 + 16 j, chunk lt % 8.
+// Rows behind the tile's last repeat a token: an MMA row depends on its own row
+// alone, and theirs are not written.
+struct Rows {
+  const uint16_t* p[8];
+  const uint16_t* any;
+  int col, K;
+  bool none;
+
+  __device__ __forceinline__ Rows(const uint16_t* rows, const uint16_t* any_, const int (&tok)[8], int K_, int lt, int step0)
+      : any(any_), K(K_), none(rows == nullptr) {
+    col = step0 * kStep + 8 * (lt & 7);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) p[j] = none ? any : rows + (size_t)(unsigned)tok[j] * (unsigned)K + col;
+  }
+  __device__ __forceinline__ void load(uint32_t dst, int steps) {
+    if (!none && col - (col & (kStep - 1)) + kStep <= K) {   // all but a matrix's ragged last step
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        cp16(dst + 2048u * j, p[j]);
+        p[j] += steps * kStep;
+      }
+    } else {
+      const int bytes = !none && col < K ? 16 : 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) cp16(dst + 2048u * j, bytes ? p[j] : any, bytes);
+    }
+    col += steps * kStep;
+  }
+};
+
+__device__ __forceinline__ void tile_tokens(int (&tok)[8], const TileArgs& a, const Unit& un, int lt) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    tok[j] = max(token_of(a.token_of_row, un.row0 + min((lt >> 3) + 16 * j, un.rows - 1), a.T), 0);
+}
+
+// ---------------------------------------------------------------------------
+// first product
+// ---------------------------------------------------------------------------
 // RB: 64-wide blocks of the rank (R <= 64 * RB).
 template <int RB>
-constexpr int tile_smem() { return 1024 + kStages * (kXBytes + RB * 8192) + RB * 2 * 16384; }
+struct Shrink {
+  static constexpr uint32_t kStageBytes = kXBytes + RB * 8192;
+  static constexpr int kPerSM = RB == 1 ? 2 : 1;
+  static constexpr int kStages = RB == 1 ? 4 : 6;      // 96 KB / 192 KB
+  static constexpr int kGroups = 2;                    // of loader warps, taking steps in turn
+  static constexpr int kThreads = kGroups * kLoaders + 32;
+  static constexpr int kSmem = 1024 + kStages * kStageBytes;
+};
 
 template <int DIR, int RB>
-__global__ void __launch_bounds__(kThreads, RB == 1 ? 2 : 1) lora_tile_kernel(const TileArgs a) {
-  constexpr uint32_t kWBytes = RB * 8192, kStageBytes = kXBytes + kWBytes;
+__global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora_shrink_kernel(const TileArgs a) {
+  using L = Shrink<RB>;
+  constexpr int kStages = L::kStages, kTurn = L::kGroups, kMmaWarp = kTurn * kLoadWarps;
+  constexpr uint32_t kTmemCols = RB * 64;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bar[kStages];
+  __shared__ uint64_t full[kStages], used[kStages], sums;
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
   __shared__ Unit unit_s;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the expand's CTAs may come as SMs free up
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), csize = (int)cl.num_blocks();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int q = warp & 3, half = warp >> 2;            // TMEM lane quarter and column half of this warp
   if (warp == 0) {
-    const Unit u = find_unit(a.offsets, a.G, a.T, kTile, a.out && a.out != a.base, (int)(blockIdx.x / csize));
+    const Unit u = find_unit(a.offsets, a.G, a.T, kTile, false, (int)((gridDim.x - 1 - blockIdx.x) / csize));
     if (lane == 0) unit_s = u;
   }
-  __syncthreads();
-  const Unit un = unit_s;
-  if (un.rows == 0) return;                            // the whole cluster leaves
-  const int K1 = a.K1, K2 = a.K2, R = a.R, g = un.g;
-  const int rk = g < a.G ? rank_of(a.rank, g, R) : 0;
-
-  // this thread's chunk and its four rows of every 128 x 64 tile: a warp fills
-  // and drains the same 32 rows x 32 columns
-  const int c8 = half * 4 + (lane & 3);
-  int tok[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int m = q * 32 + (lane >> 2) + 8 * j;
-    tok[j] = m < un.rows ? token_of(a.token_of_row, un.row0 + m, a.T) : -1;
-  }
-  // output columns of this CTA, in steps
-  const int c_all = a.out ? (K2 + kStep - 1) / kStep : 0, c_per = (c_all + csize - 1) / csize;
-  const int cb = min(c_all, rank * c_per), nc = min(c_all, cb + c_per) - cb;
-
-  if (rk == 0) {                                       // no adapter: out = base
-    if (a.u && g < a.G)
-      for (int i = rank * kThreads + tid; i < un.rows * R; i += csize * kThreads) a.u[(size_t)un.row0 * R + i] = 0.f;
-    if (a.out == a.base) return;
-    for (int s = 0; s < nc; ++s) {
-      const int col = (cb + s) * kStep + 8 * c8;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (tok[j] >= 0 && col < K2) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (a.base) v = *reinterpret_cast<const uint4*>(a.base + (size_t)tok[j] * K2 + col);
-          *reinterpret_cast<uint4*>(a.out + (size_t)tok[j] * K2 + col) = v;
-        }
+  if (warp == kMmaWarp) {                              // set up while the unit is looked for
+    if (lane == 0) {
+      for (int s = 0; s < kStages; ++s) {
+        mbar_init(&full[s], kLoaders);
+        mbar_init(&used[s], 1);
+      }
+      mbar_init(&sums, 1);
+      failed = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    return;
-  }
-
-  const int rp = (rk + 15) & ~15;                      // the MMAs' N of the first product, K of the second
-  const float scale = a.scale ? a.scale[g] : 1.0f;
-  const int k_all = (K1 + kStep - 1) / kStep, k_per = (k_all + csize - 1) / csize;
-  const int kb = min(k_all, rank * k_per), nk = min(k_all, kb + k_per) - kb;
-  const int total = nk + nc;
-
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* ub = smem + kStages * kStageBytes;          // hi blocks, lo blocks; before that the partial sums
-  float* part = reinterpret_cast<float*>(ub);          // [rp][kTile]
-  const uint32_t ring = smem_u32(smem), ua = smem_u32(ub);
-
-  if (tid == 0) {
-    for (int s = 0; s < kStages; ++s) mbar_init(&bar[s], 1);
-    failed = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == 0) {
+    __syncwarp();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
                  "r"(kTmemCols)
                  : "memory");
@@ -226,169 +368,368 @@ __global__ void __launch_bounds__(kThreads, RB == 1 ? 2 : 1) lora_tile_kernel(co
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  auto free_tmem = [&]() {
+    if (warp == kMmaWarp)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  };
+  const Unit un = unit_s;
+  if (un.rows == 0) return free_tmem();                // the whole cluster leaves
+  const int K1 = a.K1, R = a.R, g = un.g;
+  const int lt = tid % kLoaders, group = tid / kLoaders;
+  int tok[8];
+  if (warp < kMmaWarp) tile_tokens(tok, a, un, lt);    // in flight with the rank and the scale
+  const int rk = rank_of(a.rank, g, R);
+  const float scale = a.scale ? __ldg(a.scale + g) : 1.0f;
+  if (rk == 0) {
+    if (DIR == 0 && a.u)
+      for (int i = rank * L::kThreads + tid; i < un.rows * R; i += csize * L::kThreads) a.u[(size_t)un.row0 * R + i] = 0.f;
+    return free_tmem();
+  }
+  const int rp = (rk + 15) & ~15;                      // the MMAs' N
+  const int k_all = (K1 + kStep - 1) / kStep, k_per = (k_all + csize - 1) / csize;
+  const int kb = min(k_all, rank * k_per), nk = min(k_all, kb + k_per) - kb;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t ring = smem_u32(smem), full_a = smem_u32(full), used_a = smem_u32(used);
 
-  // rows of the rank, 64 columns from col0 on: A's
-  auto load_rank_rows = [&](uint32_t dst, const uint16_t* w, int K, int col0) {
-    for (int i = tid; i < rp * 8; i += kThreads) {
-      const int r = i >> 3, c = i & 7, col = col0 + 8 * c;
-      const bool in = r < rk && col < K;
-      cp16(dst + place(r, c, 0), in ? w + ((size_t)g * R + r) * K + col : w, in ? 16 : 0);
-    }
-  };
-  // 64 rows from row0 on, columns of the rank: B's
-  auto load_rank_cols = [&](uint32_t dst, const uint16_t* w, int K, int row0) {
-    const int n8 = rp / 8;
-    for (int i = tid; i < 64 * n8; i += kThreads) {
-      const int n = i / n8, c = i - n * n8;
-      const int bytes = row0 + n < K ? min(max(2 * (rk - 8 * c), 0), 16) : 0;
-      cp16(dst + place(n, c, 8192), bytes ? w + ((size_t)g * K + row0 + n) * R + 8 * c : w, bytes);
-    }
-  };
-  auto load = [&](int s) {
-    if (s < total) {
-      const uint32_t st = ring + (uint32_t)(s % kStages) * kStageBytes;
-      const bool first = s < nk;
-      const uint16_t* rows = first ? a.src : a.base;
-      const int K = first ? K1 : K2;
-      const int col0 = (first ? kb + s : cb + s - nk) * kStep, col = col0 + 8 * c8;
+  if (warp < kMmaWarp) {
+    // ------------------------------------------------------------------ load
+    const uint32_t xo = place(lt >> 3, lt & 7, 0);
+    Rows rows(a.src, a.src, tok, K1, lt, kb + group);
+    Weights<RB, DIR == 0> w(a.w1, g, K1, R, rk, rp, lt, kb + group);
+    Ring<kStages> at;
+    for (int e = 0; e < group; ++e) at.next();
+    for (int s = group; s < nk; s += kTurn) {
+      if (s >= kStages) wait_bar(used_a + 8 * at.slot, at.parity ^ 1u, &failed);
+      const uint32_t st = ring + at.slot * L::kStageBytes;
+      rows.load(st + xo, kTurn);
+      w.load(st + kXBytes, xo, kTurn);
+      cp_arrive(full_a + 8 * at.slot);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool in = rows && tok[j] >= 0 && col < K;
-        cp16(st + place(q * 32 + (lane >> 2) + 8 * j, c8, 0), in ? rows + (size_t)tok[j] * K + col : a.src, in ? 16 : 0);
-      }
-      if (first == (DIR == 0)) load_rank_rows(st + kXBytes, first ? a.w1 : a.w2, K, col0);
-      else load_rank_cols(st + kXBytes, first ? a.w1 : a.w2, K, col0);
+      for (int e = 0; e < kTurn; ++e) at.next();
     }
-    cp_commit();
-  };
+    wait_bar(smem_u32(&sums), 0, &failed);             // every MMA has read the ring
+  } else {
+    // ------------------------------------------------------------------ MMAs
+    // Its instructions are the step's critical path: descriptors are built once
+    // and moved by additions.
+    const uint32_t go = elect_one(), id = idesc(rp, 0, DIR);
+    Ring<kStages> at;
+    const uint64_t dx0 = smem_desc(ring);
+    const uint64_t dw0 = DIR ? desc_mn(ring + kXBytes, 8192) : smem_desc(ring + kXBytes);
+    constexpr uint32_t kPer = DIR ? 2048 >> 4 : 2;     // 16 contraction indices on in the weights
+#pragma unroll 1
+    for (int s = 0; s < nk; ++s) {
+      wait_bar(full_a + 8 * at.slot, at.parity, &failed);
+      fence_async();
+      const uint32_t off = at.slot * (L::kStageBytes >> 4);
+#pragma unroll
+      for (int kk = 0; kk < kStep / 16; ++kk) mma_ss(tmem, dx0 + off + 2 * kk, dw0 + off + kPer * kk, id, (s | kk) != 0, go);
+      commit_at(used_a + 8 * at.slot, go);
+      at.next();
+    }
+    commit_at(smem_u32(&sums), go);
+  }
 
-  load(0);
-  load(1);
-  for (int s = 0; s <= total; ++s) {
-    cp_wait<1>();                                      // this thread's copies of step s have landed
-    if (s == nk) {
-      // ---- the partial sums of the cluster become the second product's operand --------
-      if (nk > 0) wait_bar(&bar[(nk - 1) % kStages], (uint32_t)((nk - 1) / kStages) & 1u, &failed);
-      tc_fence_after();
-      float f[RB * 4][8];
+  // ---- sums: this thread's row, eight rank columns at a time ---------------------------
+  const int q = warp & 3, half = warp >> 2, m = q * 32 + lane, n8 = rp / 8;
+  float4* part = reinterpret_cast<float4*>(smem);      // [rp / 4][kTile][4], in the ring's place
+  const bool mine = m < un.rows && warp < kMmaWarp;
+  const size_t grow = (size_t)(un.row0 + m);
+  tc_fence_after();
+  auto write = [&](int i, float (&f)[8]) {
+    const int c0 = 8 * i;
+    if (!mine || c0 >= R) return;
 #pragma unroll
-      for (int i = 0; i < RB * 4; ++i) {
-        const int c0 = half * (rp / 2) + 8 * i;
-        if (8 * i < rp / 2) {
-          if (nk > 0) {
-            tmem_ld8(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c0, f[i]);
-          } else {
+    for (int e = 0; e < 8; ++e)
+      if (c0 + e >= rk) f[e] = 0.0f;
+    if (DIR == 0 && a.u) {
+      float4* up = reinterpret_cast<float4*>(a.u + grow * R + c0);
+      up[0] = make_float4(f[0], f[1], f[2], f[3]);
+      up[1] = make_float4(f[4], f[5], f[6], f[7]);
+    }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[i][e] = 0.0f;
-          }
-          if (csize > 1) {
+    for (int e = 0; e < 8; ++e) f[e] *= scale;
+    uint4 hi, lo;
+    split8(f, hi, lo);
+    uint16_t* sp = a.split + grow * (DIR ? 4 : 2) * R + c0;
+    *reinterpret_cast<uint4*>(sp) = hi;
+    *reinterpret_cast<uint4*>(sp + R) = lo;
+    if (DIR == 1 && a.u_in) {
+      const float4* up = reinterpret_cast<const float4*>(a.u_in + grow * R + c0);
+      const float4 u0 = __ldg(up), u1 = __ldg(up + 1);
+      float w[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) part[(c0 + e) * kTile + q * 32 + lane] = f[i][e];
-          }
-        }
+      for (int e = 0; e < 8; ++e)
+        if (c0 + e >= rk) w[e] = 0.0f;
+      split8(w, hi, lo);
+      *reinterpret_cast<uint4*>(sp + 2 * R) = hi;
+      *reinterpret_cast<uint4*>(sp + 3 * R) = lo;
+    }
+  };
+  if (csize == 1) {
+    if (warp < kMmaWarp)
+      for (int i = half; i < n8; i += 2) {
+        float f[8];
+        tmem_ld8(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(8 * i), f);
+        write(i, f);
       }
-      if (csize > 1) {
-        cl.sync();
+  } else {
+    if (warp < kMmaWarp)
+      for (int i = half; i < n8; i += 2) {
+        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (nk > 0) tmem_ld8(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(8 * i), f);
+        part[2 * i * kTile + m] = make_float4(f[0], f[1], f[2], f[3]);
+        part[(2 * i + 1) * kTile + m] = make_float4(f[4], f[5], f[6], f[7]);
+      }
+    cl.sync();
+    if (warp < kMmaWarp)
+      for (int i = rank + csize * half; i < n8; i += 2 * csize) {
+        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int cc = 0; cc < csize; cc += 4) {        // four CTAs' loads in flight, added in rank order
+          float4 v[4][2];
 #pragma unroll
-        for (int i = 0; i < RB * 4; ++i) {
-          const int c0 = half * (rp / 2) + 8 * i;
-          if (8 * i < rp / 2) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[i][e] = 0.0f;
-            for (int c = 0; c < csize; ++c) {
-              const float* p = cl.map_shared_rank(part, c) + c0 * kTile + q * 32 + lane;
-#pragma unroll
-              for (int e = 0; e < 8; ++e) f[i][e] += p[e * kTile];
+          for (int c = 0; c < 4; ++c) {
+            v[c][0] = v[c][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (cc + c < csize) {
+              const float4* p = cl.map_shared_rank(part, cc + c) + 2 * i * kTile + m;
+              v[c][0] = p[0];
+              v[c][1] = p[kTile];
             }
           }
-        }
-        cl.sync();                                     // every CTA has read; the operand takes the place
-      }
-      const int m = q * 32 + lane;
-      float* urow = a.u && rank == 0 && m < un.rows ? a.u + (size_t)(un.row0 + m) * R : nullptr;
 #pragma unroll
-      for (int i = 0; i < RB * 4; ++i) {
-        const int c0 = half * (rp / 2) + 8 * i;
-        if (8 * i < rp / 2) {
-          float v[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            if (c0 + e >= rk) f[i][e] = 0.0f;
-            v[e] = f[i][e] * scale;
+          for (int c = 0; c < 4; ++c) {
+            f[0] += v[c][0].x; f[1] += v[c][0].y; f[2] += v[c][0].z; f[3] += v[c][0].w;
+            f[4] += v[c][1].x; f[5] += v[c][1].y; f[6] += v[c][1].z; f[7] += v[c][1].w;
           }
-          if (urow && c0 < R) {
-            float4* up = reinterpret_cast<float4*>(urow + c0);
-            up[0] = DIR ? make_float4(v[0], v[1], v[2], v[3]) : make_float4(f[i][0], f[i][1], f[i][2], f[i][3]);
-            up[1] = DIR ? make_float4(v[4], v[5], v[6], v[7]) : make_float4(f[i][4], f[i][5], f[i][6], f[i][7]);
-          }
-          uint4 hi, lo;
-          split8(v, hi, lo);
-          const uint32_t o = place(m, c0 / 8, 16384);
-          *reinterpret_cast<uint4*>(ub + o) = hi;
-          *reinterpret_cast<uint4*>(ub + RB * 16384 + o) = lo;
         }
+        write(i, f);
       }
-      if (urow && half == 0)
-        for (int c = rp; c < R; c += 4) *reinterpret_cast<float4*>(urow + c) = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    fence_async();
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    if (tid == 0 && s < total) {
-      const uint32_t st = ring + (uint32_t)(s % kStages) * kStageBytes, w = st + kXBytes;
-      if (s < nk) {
-        const uint32_t id = idesc(rp, 0, DIR);
-#pragma unroll
-        for (int kk = 0; kk < kStep / 16; ++kk)
-          tc_mma(tmem, smem_desc(st) + 2 * kk, DIR ? desc_mn(w + 2048 * kk, 8192) : smem_desc(w) + 2 * kk, id,
-                 (s | kk) != 0);
-      } else {
-        const uint32_t id = idesc(kStep, 0, DIR), d = tmem + 128 + 64 * (uint32_t)((s - nk) & 1);
-        for (int kk = 0; kk < rp / 16; ++kk) {
-          const uint64_t db = DIR ? desc_mn(w + 2048 * kk, 8192) : smem_desc(w + (kk >> 2) * 8192) + 2 * (kk & 3);
-          const uint64_t dh = smem_desc(ua + (kk >> 2) * 16384) + 2 * (kk & 3);
-          const uint64_t dl = smem_desc(ua + RB * 16384 + (kk >> 2) * 16384) + 2 * (kk & 3);
-          tc_mma(d, dh, db, id, kk != 0);
-          tc_mma(d, dl, db, id, 1);
-        }
-      }
-      tc_commit(&bar[s % kStages]);
-    }
-    __syncwarp();
-    if (s > 0) wait_bar(&bar[(s - 1) % kStages], (uint32_t)((s - 1) / kStages) & 1u, &failed);
-    if (s > nk) {
-      // ---- drain the output of step s - 1: base plus product, one rounding -------------
-      const int o = s - 1 - nk;
-      uint8_t* xt = smem + (size_t)((s - 1) % kStages) * kStageBytes;
-      tc_fence_after();
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float d[8], b[8];
-        tmem_ld8(tmem + ((uint32_t)(q * 32) << 16) + 128u + 64u * (uint32_t)(o & 1) + (uint32_t)(half * 32 + 8 * c), d);
-        uint4* p = reinterpret_cast<uint4*>(xt + place(q * 32 + lane, half * 4 + c, 0));
-        unpack8(*p, b);
-        *p = make_uint4(pack2(b[0] + d[0], b[1] + d[1]), pack2(b[2] + d[2], b[3] + d[3]),
-                        pack2(b[4] + d[4], b[5] + d[5]), pack2(b[6] + d[6], b[7] + d[7]));
-      }
-      __syncwarp();
-      const int col = (cb + o) * kStep + 8 * c8;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (tok[j] >= 0 && col < K2)
-          *reinterpret_cast<uint4*>(a.out + (size_t)tok[j] * K2 + col) =
-              *reinterpret_cast<const uint4*>(xt + place(q * 32 + (lane >> 2) + 8 * j, c8, 0));
-      __syncwarp();
-    }
-    load(s + 2);
+    cl.sync();                                         // partial sums stay until every CTA has read them
   }
-  cp_wait<0>();
+  if (DIR == 0 && a.u && rank == 0 && mine && half == 0)
+    for (int c = rp; c < R; c += 4) *reinterpret_cast<float4*>(a.u + grow * R + c) = make_float4(0.f, 0.f, 0.f, 0.f);
   tc_fence_before();
   __syncthreads();
+  tc_fence_after();
+  free_tmem();
+}
+
+// ---------------------------------------------------------------------------
+// second product
+// ---------------------------------------------------------------------------
+template <int RB>
+struct Expand {
+  static constexpr uint32_t kStageBytes = kXBytes + RB * 8192;
+  static constexpr int kPerSM = RB == 1 ? 2 : 1;
+  static constexpr int kStages = RB == 1 ? 3 : 4;
+  static constexpr uint32_t kOperand = RB * 2 * 16384; // hi blocks, lo blocks
+  static constexpr int kOuts = 4;                      // 64-column outputs in TMEM
+  static constexpr int kDrainWarps = 8;                // two groups, taking steps in turn
+  static constexpr int kThreads = 32 * (kDrainWarps + 1 + kLoadWarps);
+  static constexpr int kSmem = 1024 + kStages * kStageBytes + kOperand;
+};
+
+template <int DIR, int RB>
+__global__ void __launch_bounds__(Expand<RB>::kThreads, Expand<RB>::kPerSM) lora_expand_kernel(const TileArgs a) {
+  using L = Expand<RB>;
+  constexpr int kStages = L::kStages, kDrainWarps = L::kDrainWarps, kOuts = L::kOuts;
+  constexpr uint32_t kTmemCols = 64 * kOuts;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[kStages], used[kStages], operand, out_full[kOuts], out_free[kOuts];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed;
+  __shared__ Unit unit_s;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int index = (int)(gridDim.x - 1 - blockIdx.x), part = index % a.parts;
   if (warp == 0) {
-    tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    const Unit u = find_unit(a.offsets, a.G, a.T, kTile, a.out != a.base, index / a.parts);
+    if (lane == 0) unit_s = u;
   }
+  if (warp == kDrainWarps) {
+    if (lane == 0) {
+      for (int s = 0; s < kStages; ++s) {
+        mbar_init(&full[s], kLoaders);
+        mbar_init(&used[s], kDrainWarps / 2);
+      }
+      mbar_init(&operand, kLoaders);
+      for (int i = 0; i < kOuts; ++i) {
+        mbar_init(&out_full[i], 1);
+        mbar_init(&out_free[i], kDrainWarps / 2);
+      }
+      failed = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  auto free_tmem = [&]() {
+    // the launch does not end before the shrink has, whatever its CTAs had to do
+    if (blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (warp == kDrainWarps)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  };
+  const Unit un = unit_s;
+  const int K2 = a.K2, R = a.R, g = un.g;
+  const int c_all = (K2 + kStep - 1) / kStep, c_per = (c_all + a.parts - 1) / a.parts;
+  const int cb = min(c_all, part * c_per), nc = min(c_all, cb + c_per) - cb;
+  if (un.rows == 0 || nc == 0) return free_tmem();
+  int tok[8];
+  const int q = warp & 3, half = warp >> 2;            // drain warps: TMEM lane quarter and group
+  if (warp > kDrainWarps) {
+    tile_tokens(tok, a, un, tid - 32 * (kDrainWarps + 1));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {                      // the rows this lane writes: q*32 + lane/8 + 4j
+      const int r = q * 32 + (lane >> 3) + 4 * j;
+      tok[j] = r < un.rows ? token_of(a.token_of_row, un.row0 + r, a.T) : -1;
+    }
+  }
+  const int rk = g < a.G ? rank_of(a.rank, g, R) : 0;
+  if (rk == 0) {                                       // no adapter: out = base
+    if (a.out == a.base) return free_tmem();
+    const int v8 = (min(K2, (cb + nc) * kStep) - cb * kStep) / 8;
+    for (int m = warp; m < un.rows; m += L::kThreads / 32) {
+      const int t = token_of(a.token_of_row, un.row0 + m, a.T);
+      if (t < 0) continue;
+      const size_t at = (size_t)t * K2 + cb * kStep;
+      for (int c = lane; c < v8; c += 32) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (a.base) v = *reinterpret_cast<const uint4*>(a.base + at + 8 * c);
+        *reinterpret_cast<uint4*>(a.out + at + 8 * c) = v;
+      }
+    }
+    return free_tmem();
+  }
+  const int rp = (rk + 15) & ~15;                      // the MMAs' K
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t ring = smem_u32(smem), full_a = smem_u32(full), used_a = smem_u32(used);
+  const uint32_t op = ring + kStages * L::kStageBytes;
+
+  if (warp > kDrainWarps) {
+    // ------------------------------------------------------------------ load
+    const int l = tid - 32 * (kDrainWarps + 1);
+    const uint32_t xo = place(l >> 3, l & 7, 0);
+    Rows rows(a.base, a.w2, tok, K2, l, cb);
+    Weights<RB, DIR == 1> w(a.w2, g, K2, R, rk, rp, l, cb);
+    Ring<kStages> at;
+    auto step = [&]() {
+      const uint32_t st = ring + at.slot * L::kStageBytes;
+      rows.load(st + xo, 1);
+      w.load(st + kXBytes, xo, 1);
+      cp_arrive(full_a + 8 * at.slot);
+      at.next();
+    };
+    // base and weights do not depend on the shrink: they go first
+    const int ahead = min(nc, kStages);
+    for (int s = 0; s < ahead; ++s) step();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int n8 = min(rp, R) / 8;                     // chunks in memory; zeros behind them up to rp / 8
+#pragma unroll
+    for (int e = 0; e < RB; ++e) {
+      const int c = (l & 7) + 8 * e;
+      if (c < rp / 8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int m = (l >> 3) + 16 * j;
+          const uint16_t* sp = a.split + (size_t)(un.row0 + min(m, un.rows - 1)) * (DIR ? 4 : 2) * R + 8 * c;
+          const int bytes = c < n8 ? 16 : 0;
+          cp16(op + xo + 2048u * j + 16384u * e, bytes ? sp : a.split, bytes);
+          cp16(op + xo + 2048u * j + 16384u * (e + RB), bytes ? sp + R : a.split, bytes);
+        }
+      }
+    }
+    cp_arrive(smem_u32(&operand));
+    for (int s = ahead; s < nc; ++s) {
+      wait_bar(used_a + 8 * at.slot, at.parity ^ 1u, &failed);
+      step();
+    }
+  } else if (warp == kDrainWarps) {
+    // ------------------------------------------------------------------ MMAs
+    const uint32_t go = elect_one(), id = idesc(kStep, 0, DIR);
+    Ring<kStages> at;
+    const uint64_t du = smem_desc(op);
+    const uint64_t dw0 = DIR ? desc_mn(ring + kXBytes, 8192) : smem_desc(ring + kXBytes);
+    const uint32_t of = smem_u32(out_full), fr = smem_u32(out_free);
+    wait_bar(smem_u32(&operand), 0, &failed);
+#pragma unroll 1
+    for (int o = 0; o < nc; ++o) {
+      const int buf = o % kOuts;
+      wait_bar(full_a + 8 * at.slot, at.parity, &failed);
+      if (o >= kOuts) {
+        wait_bar(fr + 8 * buf, (uint32_t)(o / kOuts - 1) & 1u, &failed);
+        tc_fence_after();
+      }
+      fence_async();
+      const uint64_t dw = dw0 + at.slot * (L::kStageBytes >> 4);
+      const uint32_t d = tmem + 64 * (uint32_t)buf;
+#pragma unroll 1
+      for (int kk = 0; 16 * kk < rp; ++kk) {
+        const uint64_t db = dw + (DIR ? (2048 >> 4) * kk : (kk >> 2) * (8192 >> 4) + 2 * (kk & 3));
+        const uint64_t da = du + (kk >> 2) * (16384 >> 4) + 2 * (kk & 3);
+        mma_ss(d, da, db, id, kk != 0, go);
+        mma_ss(d, da + RB * (16384 >> 4), db, id, 1, go);
+      }
+      commit_at(of + 8 * buf, go);
+      at.next();
+    }
+  } else {
+    // ------------------------------------------------------------------ outputs
+    // base (in the ring) plus product, one rounding.  The two groups of four
+    // warps take alternate steps, so that one's latencies hide behind the other's
+    const int m = q * 32 + lane;
+    const uint32_t ro = place(q * 32 + (lane >> 3), lane & 7, 0), mo = place(m, 0, 0);
+    Ring<kStages> at;
+    if (half) at.next();
+    const uint32_t of = smem_u32(out_full);
+    for (int o = half; o < nc; o += 2) {
+      const int buf = o % kOuts;
+      uint8_t* xt = smem + (size_t)at.slot * L::kStageBytes;
+      wait_bar(of + 8 * buf, (uint32_t)(o / kOuts) & 1u, &failed);
+      wait_bar(full_a + 8 * at.slot, at.parity, &failed);
+      tc_fence_after();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t d[2][16];
+        tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + 64u * (uint32_t)buf + 32u * h, d[0], d[1]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float b[8];
+          uint4* p = reinterpret_cast<uint4*>(xt + (mo ^ (uint32_t)((4 * h + c) << 4)));
+          unpack8(*p, b);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) b[e] += __uint_as_float(d[c >> 1][(c & 1) * 8 + e]);
+          *p = make_uint4(pack2(b[0], b[1]), pack2(b[2], b[3]), pack2(b[4], b[5]), pack2(b[6], b[7]));
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&out_free[buf]);
+      const int col = (cb + o) * kStep + 8 * (lane & 7);
+      if (col < K2) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (tok[j] >= 0)
+            *reinterpret_cast<uint4*>(a.out + (size_t)(unsigned)tok[j] * (unsigned)K2 + col) =
+                *reinterpret_cast<const uint4*>(xt + ((ro + 512u * j) ^ ((j & 1) << 6)));
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&used[at.slot]);
+      at.next();
+      at.next();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  free_tmem();
 }
 
 // ---------------------------------------------------------------------------
@@ -396,7 +737,7 @@ __global__ void __launch_bounds__(kThreads, RB == 1 ? 2 : 1) lora_tile_kernel(co
 // ---------------------------------------------------------------------------
 struct DwArgs {
   const uint16_t* src[2];                              // x [T, H], dy [T, N]
-  const float* f[2];                                   // v [T, R], u [T, R]
+  const uint16_t* split;                               // [T][v hi, v lo, u hi, u lo][R]
   uint16_t* out[2];                                    // da [G, R, H], db [G, N, R]
   const float* scale;
   const int32_t *rank, *offsets, *token_of_row;
@@ -404,30 +745,41 @@ struct DwArgs {
   int T, G, R;
 };
 
+// A step is 32 rows: 8 KB of x or dy and RB x 8 KB of the factor's two halves.
 template <int RB>
-constexpr int dw_smem() { return 1024 + kStages * (kXBytes + RB * 2 * 8192); }
+struct Dw {
+  static constexpr int kRows = 32;
+  static constexpr uint32_t kSrcBytes = kRows * kTile * 2, kHalf = RB * kRows * 128;
+  static constexpr uint32_t kStageBytes = kSrcBytes + 2 * kHalf;
+  static constexpr int kPerSM = RB == 1 ? 4 : 2;
+  static constexpr int kStages = RB == 1 ? 3 : 4;      // 48 KB / 96 KB
+  static constexpr int kSmem = 1024 + kStages * kStageBytes;
+};
+
+constexpr int kDwThreads = kLoaders + 32;              // four warps load and then drain, one issues the MMAs
 
 template <int RB>
-__global__ void __launch_bounds__(kThreads, RB == 1 ? 2 : 1) lora_dw_kernel(const DwArgs a) {
-  constexpr uint32_t kStageBytes = kXBytes + RB * 2 * 8192;
+__global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(const DwArgs a) {
+  using D = Dw<RB>;
+  constexpr int kStages = D::kStages, kRows = D::kRows;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bar[kStages];
+  __shared__ uint64_t full[kStages], used[kStages], sums;
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), csize = (int)cl.num_blocks();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q = warp & 3, half = warp >> 2;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int tilesA = (a.M[0] + kTile - 1) / kTile;
   const int unit = (int)(blockIdx.x / csize), g = blockIdx.y;
   const int which = unit >= tilesA, m0 = (which ? unit - tilesA : unit) * kTile, M = a.M[which];
   const int R = a.R, rk = rank_of(a.rank, g, R);
   const int r0 = min(max(a.offsets[g], 0), a.T), r1 = min(max(a.offsets[g + 1], 0), a.T);
   uint16_t* out = a.out[which];
-  const int m = m0 + q * 32 + lane;                    // this thread's column of src (TMEM lane)
+  const int m = m0 + tid;                              // a drain thread's column of src (TMEM lane)
 
   // eight rank columns from c0 on of column m
   auto store = [&](int c0, const float (&v)[8]) {
-    if (m >= M || c0 >= R) return;
+    if (tid >= kTile || m >= M || c0 >= R) return;
     if (which) {
       *reinterpret_cast<uint4*>(out + ((size_t)g * M + m) * R + c0) =
           make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
@@ -438,20 +790,28 @@ __global__ void __launch_bounds__(kThreads, RB == 1 ? 2 : 1) lora_dw_kernel(cons
   };
   const float zero8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   const int rp = r1 > r0 ? (rk + 15) & ~15 : 0;
-  for (int c = rp / 8 + rank * 2 + half; c < R / 8; c += 2 * csize) store(8 * c, zero8);
-  if (rp == 0) return;                                 // the whole cluster leaves
+  for (int c = rp / 8 + rank; c < R / 8; c += csize) store(8 * c, zero8);
+  if (rp == 0) {                                       // the whole cluster leaves
+    // but the launch does not end before the one that it depends on
+    if (blockIdx.x == 0 && blockIdx.y == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
 
-  const int s_all = (r1 - r0 + kStep - 1) / kStep, s_per = (s_all + csize - 1) / csize;
+  const int s_all = (r1 - r0 + kRows - 1) / kRows, s_per = (s_all + csize - 1) / csize;
   const int sb = min(s_all, rank * s_per), ns = min(s_all, sb + s_per) - sb;
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const uint32_t ring = smem_u32(smem);
+  const uint32_t ring = smem_u32(smem), full_a = smem_u32(full), used_a = smem_u32(used);
   if (tid == 0) {
-    for (int s = 0; s < kStages; ++s) mbar_init(&bar[s], 1);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], kLoaders);
+      mbar_init(&used[s], 1);
+    }
+    mbar_init(&sums, 1);
     failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 0) {
+  if (warp == kLoadWarps) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
                  "r"(128)
                  : "memory");
@@ -462,173 +822,204 @@ __global__ void __launch_bounds__(kThreads, RB == 1 ? 2 : 1) lora_dw_kernel(cons
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  // 64 rows x 128 columns of src per step: this thread's chunk and four rows
-  const int ch = tid & 15, col = m0 + 8 * ch;
-  const uint16_t* src = a.src[which];
-  const float* fsrc = a.f[which];
-  int tok[4];                                          // rows of the next load
-  auto load_tok = [&](int s) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int row = r0 + (sb + s) * kStep + (tid >> 4) + 16 * j;
-      tok[j] = s < ns && row < r1 ? token_of(a.token_of_row, row, a.T) : -1;
-    }
-  };
-  auto load_x = [&](int s) {
-    if (s < ns) {
-      const uint32_t st = ring + (uint32_t)(s % kStages) * kStageBytes;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool in = tok[j] >= 0 && col < M;
-        cp16(st + place((tid >> 4) + 16 * j, ch, 8192), in ? src + (size_t)tok[j] * M + col : src, in ? 16 : 0);
-      }
-    }
-    cp_commit();
-  };
-  // the factor's rows: 64 x rp fp32, eight columns per item
-  const int n8 = rp / 8;
-  float fr[RB * 2][8];
-  auto load_f = [&](int s) {
-#pragma unroll
-    for (int i = 0; i < RB * 2; ++i) {
-      const int it = tid + i * kThreads, kr = it / n8, c = it - kr * n8;
-      const int row = r0 + (sb + s) * kStep + kr;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) fr[i][e] = 0.0f;
-      if (s < ns && kr < kStep && row < r1 && 8 * c < R &&
-          (a.token_of_row == nullptr || (unsigned)__ldg(a.token_of_row + row) < (unsigned)a.T)) {
-        const float4* p = reinterpret_cast<const float4*>(fsrc + (size_t)row * R + 8 * c);
-        const float4 lo = __ldg(p), hi = __ldg(p + 1);
-        const float t[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (8 * c + e < rk) fr[i][e] = t[e];
-      }
-    }
-  };
-  auto store_f = [&](int s) {
-    if (s >= ns) return;
-    uint8_t* w = smem + (size_t)(s % kStages) * kStageBytes + kXBytes;
-#pragma unroll
-    for (int i = 0; i < RB * 2; ++i) {
-      const int it = tid + i * kThreads, kr = it / n8, c = it - kr * n8;
-      if (kr >= kStep) continue;
-      uint4 hi, lo;
-      split8(fr[i], hi, lo);
-      const uint32_t o = place(kr, c, 8192);
-      *reinterpret_cast<uint4*>(w + o) = hi;
-      *reinterpret_cast<uint4*>(w + RB * 8192 + o) = lo;
-    }
-  };
-
-  load_tok(0);
-  load_x(0);
-  load_tok(1);
-  load_x(1);
-  load_f(0);
-  store_f(0);
-  load_f(1);
-  store_f(1);
-  load_f(2);
-  load_tok(2);
-  for (int s = 0; s < ns; ++s) {
-    cp_wait<1>();
-    fence_async();
-    __syncthreads();
-    if (tid == 0) {
-      const uint32_t st = ring + (uint32_t)(s % kStages) * kStageBytes, w = st + kXBytes;
+  if (warp == kLoadWarps) {
+    // ------------------------------------------------------------------ MMAs
+    {
+      const uint32_t go = elect_one();
       const uint32_t id = idesc(rp, 1, 1);
+      const uint64_t dx0 = desc_mn(ring, kRows * 128), dw0 = desc_mn(ring + D::kSrcBytes, kRows * 128);
+      Ring<kStages> at;
+#pragma unroll 1
+      for (int s = 0; s < ns; ++s) {
+        wait_bar(full_a + 8 * at.slot, at.parity, &failed);
+        fence_async();
+        const uint32_t off = at.slot * (D::kStageBytes >> 4);
 #pragma unroll
-      for (int kk = 0; kk < kStep / 16; ++kk) {
-        const uint64_t da = desc_mn(st + 2048 * kk, 8192);
-        tc_mma(tmem, da, desc_mn(w + 2048 * kk, 8192), id, (s | kk) != 0);
-        tc_mma(tmem, da, desc_mn(w + RB * 8192 + 2048 * kk, 8192), id, 1);
+        for (int kk = 0; kk < kRows / 16; ++kk) {
+          const uint64_t da = dx0 + off + kk * (2048 >> 4), dw = dw0 + off + kk * (2048 >> 4);
+          mma_ss(tmem, da, dw, id, (s | kk) != 0, go);
+          mma_ss(tmem, da, dw + (D::kHalf >> 4), id, 1, go);
+        }
+        commit_at(used_a + 8 * at.slot, go);
+        at.next();
       }
-      tc_commit(&bar[s % kStages]);
+      commit_at(smem_u32(&sums), go);
     }
     __syncwarp();
-    if (s > 0) wait_bar(&bar[(s - 1) % kStages], (uint32_t)((s - 1) / kStages) & 1u, &failed);
-    store_f(s + 2);
-    load_x(s + 2);
-    load_f(s + 3);
-    load_tok(s + 3);
+  } else {
+    // ------------------------------------------------------------------ loaders
+    // 32 rows x 128 columns of src per step: this thread's chunk of rows
+    // tid/16 + 8j; the factor's two halves: rows tid/8 + 16j, chunk tid%8 (+ 8)
+    const int ch = tid & 15, col = m0 + 8 * ch, xr = tid >> 4, fr = tid >> 3, fc = tid & 7;
+    uint32_t xo[2], fo = D::kSrcBytes + place(fr, fc, 0);
+    xo[0] = place(xr, ch, kRows * 128);                // + 2048 for rows 16 on
+    xo[1] = place(xr + 8, ch, kRows * 128);
+    const uint16_t* src = a.src[which];
+    const int n8 = min(rp, R) / 8;                     // chunks in memory; zeros behind them up to rp / 8
+    const uint16_t* fp = a.split + ((size_t)(r0 + sb * kRows + fr) * 4 + 2 * which) * R + 8 * fc;
+    const int first = r0 + sb * kRows;
+    const int xbytes = col < M ? 16 : 0;
+    const uint16_t* xsrc = xbytes ? src + col : src;
+    // tokens: lane l holds row l of each of four steps, loaded four steps ahead
+    int cur[4], nxt[4];
+    auto load_tok = [&](int (&t)[4], int s) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = first + (s + i) * kRows + lane;
+        t[i] = s + i < ns && row < r1 ? (a.token_of_row ? __ldg(a.token_of_row + row) : row) : -1;
+      }
+    };
+    load_tok(cur, 0);
+    asm volatile("griddepcontrol.wait;" ::: "memory"); // the factors come from the shrink
+    Ring<kStages> at;
+    for (int s0 = 0; s0 < ns; s0 += 4) {
+      load_tok(nxt, s0 + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int s = s0 + e;
+        if (s >= ns) break;
+        if (s >= kStages) wait_bar(used_a + 8 * at.slot, at.parity ^ 1u, &failed);
+        const uint32_t st = ring + at.slot * D::kStageBytes;
+        const int row = first + s * kRows;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int t = __shfl_sync(kFull, cur[e], xr + 8 * j);
+          const bool in = (unsigned)t < (unsigned)a.T;
+          cp16(st + xo[j & 1] + 2048u * (j >> 1), in ? xsrc + (size_t)(unsigned)t * (unsigned)M : src, in ? xbytes : 0);
+        }
+#pragma unroll
+        for (int i = 0; i < RB; ++i) {
+          const int c = fc + 8 * i;
+          if (c < rp / 8) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int bytes = row + fr + 16 * j < r1 && c < n8 ? 16 : 0;
+              const uint16_t* p = bytes ? fp + (size_t)(64 * j) * R + 64 * i : a.split;   // 16 rows of 4 R
+              const uint32_t o = st + fo + (uint32_t)(i * kRows * 128 + j * 2048);
+              cp16(o, p, bytes);
+              cp16(o + D::kHalf, bytes ? p + R : p, bytes);
+            }
+          }
+        }
+        fp += (size_t)kRows * 4 * R;
+        cp_arrive(full_a + 8 * at.slot);
+        at.next();
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) cur[e] = nxt[e];
+    }
+    wait_bar(smem_u32(&sums), 0, &failed);             // every MMA has read the ring
+    tc_fence_after();
   }
-  cp_wait<0>();
-  if (ns > 0) wait_bar(&bar[(ns - 1) % kStages], (uint32_t)((ns - 1) / kStages) & 1u, &failed);
-  tc_fence_after();
   __syncthreads();                                     // the ring is free: partial sums take its place
-  float* part = reinterpret_cast<float*>(smem);        // [rp][kTile]
+  float4* part = reinterpret_cast<float4*>(smem);      // [rp / 4][kTile][4]
   const float scale = which && a.scale ? a.scale[g] : 1.0f;
-  for (int c = half; c < n8; c += 2) {
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (ns > 0) tmem_ld8(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(8 * c), v);
-    if (csize > 1) {
+  if (warp < kLoadWarps) {
+    for (int c = 0; c < rp / 8; ++c) {
+      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (ns > 0) tmem_ld8(tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(8 * c), v);
+      if (csize > 1) {
+        part[(2 * c) * kTile + tid] = make_float4(v[0], v[1], v[2], v[3]);
+        part[(2 * c + 1) * kTile + tid] = make_float4(v[4], v[5], v[6], v[7]);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) part[(8 * c + e) * kTile + q * 32 + lane] = v[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 8 * c + e < rk ? v[e] * scale : 0.0f;
-      store(8 * c, v);
+        for (int e = 0; e < 8; ++e) v[e] = 8 * c + e < rk ? v[e] * scale : 0.0f;
+        store(8 * c, v);
+      }
     }
   }
   if (csize > 1) {
     cl.sync();
-    for (int c = rank * 2 + half; c < n8; c += 2 * csize) {
-      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      for (int p = 0; p < csize; ++p) {
-        const float* rp_ = cl.map_shared_rank(part, p) + 8 * c * kTile + q * 32 + lane;
+    if (warp < kLoadWarps) {
+      for (int c = rank; c < rp / 8; c += csize) {
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int pc = 0; pc < csize; pc += 4) {        // four CTAs' loads in flight, added in rank order
+          float4 w[4][2];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += rp_[e * kTile];
+          for (int i = 0; i < 4; ++i) {
+            w[i][0] = w[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (pc + i < csize) {
+              const float4* p = cl.map_shared_rank(part, pc + i) + 2 * c * kTile + tid;
+              w[i][0] = p[0];
+              w[i][1] = p[kTile];
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            v[0] += w[i][0].x; v[1] += w[i][0].y; v[2] += w[i][0].z; v[3] += w[i][0].w;
+            v[4] += w[i][1].x; v[5] += w[i][1].y; v[6] += w[i][1].z; v[7] += w[i][1].w;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = 8 * c + e < rk ? v[e] * scale : 0.0f;
+        store(8 * c, v);
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 8 * c + e < rk ? v[e] * scale : 0.0f;
-      store(8 * c, v);
     }
     cl.sync();                                         // partial sums stay until every CTA has read them
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 0) {
+  if (warp == kLoadWarps) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(128) : "memory");
   }
 }
 
 template <class K, class A>
-zmoe_status launch_clusters(K* kernel, dim3 grid, int csize, int smem, cudaStream_t stream, const A& args,
-                            const char* what) {
+zmoe_status launch(K* kernel, dim3 grid, int threads, int csize, bool dependent, int smem, cudaStream_t stream,
+                   const A& args, const char* what) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)csize;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)csize;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent ? 2 : 1;
   ZMOE_CUDA_RET(cudaLaunchKernelEx(&cfg, kernel, args));
   return launch_status(what);
 }
 
-// CTAs per cluster: enough that `units` clusters fill the SMs' two places, no
-// more than there are steps to share.
-int cluster_size(long long units, int steps, int per_sm) {
-  int c = 1;
-  while (c < 8 && 2 * c * units <= (long long)kNumSMs * per_sm && 2 * c <= steps) c *= 2;
-  return c;
+// How many CTAs share a unit of `steps` steps: the count with the least rounds x
+// (steps of a CTA + fixed), where a round fills the `places` of the SMs and
+// `fixed` is what a CTA spends around its steps, in steps.
+int share(long long units, int steps, int places, int fixed, int fixed_shared, int most, bool powers) {
+  int best = 1;
+  long long least = -1;
+  for (int c = 1; c <= most && c <= steps; c = powers ? 2 * c : c + 1) {
+    const long long rounds = (units * c + places - 1) / places;
+    const long long cost = rounds * ((steps + c - 1) / c + (c > 1 ? fixed_shared : fixed));
+    if (least < 0 || cost < least) {
+      least = cost;
+      best = c;
+    }
+  }
+  return best;
 }
 
 template <int DIR, int RB>
-zmoe_status launch_tile(const TileArgs& a, cudaStream_t stream) {
-  zmoe_status st = allow_smem<lora_tile_kernel<DIR, RB>>();
+zmoe_status launch_tiles(TileArgs a, cudaStream_t stream) {
+  const long long units = a.T / kTile + (a.T < a.G + 1 ? a.T : a.G + 1);       // at most
+  const int tiles = (a.T + kTile - 1) / kTile + (a.T < a.G ? a.T : a.G) / 2;   // about
+  using S = Shrink<RB>;
+  using E = Expand<RB>;
+  zmoe_status st = allow_smem<lora_shrink_kernel<DIR, RB>>();
+  if (st == ZMOE_OK) st = allow_smem<lora_expand_kernel<DIR, RB>>();
   if (st != ZMOE_OK) return st;
-  const long long units = a.T / kTile + (a.T < a.G + 1 ? a.T : a.G + 1);
-  const int csize = cluster_size(units, (a.K1 + kStep - 1) / kStep, RB == 1 ? 2 : 1);
-  ZMOE_CHECK_ARG(units * csize < (1LL << 31), "lora: T=%d rows are too many for one launch", a.T);
-  return launch_clusters(lora_tile_kernel<DIR, RB>, dim3((unsigned)(units * csize)), csize, tile_smem<RB>(), stream, a,
-                         "lora_tile_kernel");
+  const int c = share(tiles, (a.K1 + kStep - 1) / kStep, kNumSMs * S::kPerSM, 2, 8, 8, true);
+  a.parts = share(tiles, (a.K2 + kStep - 1) / kStep, kNumSMs * E::kPerSM, 5, 5, 64, false);
+  ZMOE_CHECK_ARG(units * c < (1LL << 31) && units * a.parts < (1LL << 31), "lora: T=%d rows are too many for one launch",
+                 a.T);
+  st = launch(lora_shrink_kernel<DIR, RB>, dim3((unsigned)(units * c)), S::kThreads, c, false, S::kSmem, stream, a,
+              "lora_shrink_kernel");
+  if (st != ZMOE_OK || !a.out) return st;
+  return launch(lora_expand_kernel<DIR, RB>, dim3((unsigned)(units * a.parts)), E::kThreads, 1, true, E::kSmem, stream, a,
+                "lora_expand_kernel");
 }
 
 template <int RB>
@@ -636,26 +1027,27 @@ zmoe_status launch_dw(const DwArgs& a, cudaStream_t stream) {
   zmoe_status st = allow_smem<lora_dw_kernel<RB>>();
   if (st != ZMOE_OK) return st;
   const int tiles = (a.M[0] + kTile - 1) / kTile + (a.M[1] + kTile - 1) / kTile;
-  const int steps = (a.T + kStep - 1) / kStep;
-  const int csize = cluster_size((long long)tiles * a.G, steps, RB == 1 ? 2 : 1);
-  return launch_clusters(lora_dw_kernel<RB>, dim3((unsigned)(tiles * csize), (unsigned)a.G), csize, dw_smem<RB>(),
-                         stream, a, "lora_dw_kernel");
+  const int steps = (a.T + Dw<RB>::kRows - 1) / Dw<RB>::kRows;
+  const int csize = share((long long)tiles * a.G, (steps + a.G - 1) / a.G, kNumSMs * Dw<RB>::kPerSM, 2, 8, 8, true);
+  return launch(lora_dw_kernel<RB>, dim3((unsigned)(tiles * csize), (unsigned)a.G), kDwThreads, csize, true,
+                Dw<RB>::kSmem, stream, a, "lora_dw_kernel");
 }
 
 }  // namespace
 
 zmoe_status launch_tiles(const zmoe_lora_args* p, cudaStream_t stream) {
-  const TileArgs a{p->x, p->a, p->b, p->base, p->scale, p->rank, p->offsets, p->token_of_row,
-                   p->T, p->H, p->N, p->G, p->R, p->out, p->u};
-  return p->R <= 64 ? launch_tile<0, 1>(a, stream) : launch_tile<0, 2>(a, stream);
+  const TileArgs a{p->x, p->a, p->b, p->base, p->scale, p->rank, p->offsets, p->token_of_row, p->T, p->H, p->N, p->G,
+                   p->R, p->out, p->u, nullptr, reinterpret_cast<uint16_t*>(p->scratch), 1};
+  return p->R <= 64 ? launch_tiles<0, 1>(a, stream) : launch_tiles<0, 2>(a, stream);
 }
 
 zmoe_status launch_grad_tiles(const zmoe_lora_grad_args* p, cudaStream_t stream) {
-  const TileArgs a{p->dy, p->b, p->a, p->base, p->scale, p->rank, p->offsets, p->token_of_row,
-                   p->T, p->N, p->H, p->G, p->R, p->dx, p->v};
-  zmoe_status st = p->R <= 64 ? launch_tile<1, 1>(a, stream) : launch_tile<1, 2>(a, stream);
+  uint16_t* split = reinterpret_cast<uint16_t*>(p->scratch);
+  const TileArgs a{p->dy, p->b, p->a, p->base, p->scale, p->rank, p->offsets, p->token_of_row, p->T, p->N, p->H, p->G,
+                   p->R, p->dx, nullptr, p->da ? p->u : nullptr, split, 1};
+  zmoe_status st = p->R <= 64 ? launch_tiles<1, 1>(a, stream) : launch_tiles<1, 2>(a, stream);
   if (st != ZMOE_OK || !p->da) return st;
-  const DwArgs d{{p->x, p->dy}, {p->v, p->u}, {p->da, p->db}, p->scale, p->rank, p->offsets, p->token_of_row,
+  const DwArgs d{{p->x, p->dy}, split, {p->da, p->db}, p->scale, p->rank, p->offsets, p->token_of_row,
                  {p->H, p->N}, p->T, p->G, p->R};
   return p->R <= 64 ? launch_dw<1>(d, stream) : launch_dw<2>(d, stream);
 }

@@ -72,14 +72,15 @@ class CombineGradArgs(ctypes.Structure):
 class LoraArgs(ctypes.Structure):
     _fields_ = [("x", c_void_p), ("base", c_void_p), ("a", c_void_p), ("b", c_void_p), ("scale", c_void_p),
                 ("rank", c_void_p), ("offsets", c_void_p), ("token_of_row", c_void_p), ("T", c_int), ("H", c_int),
-                ("N", c_int), ("G", c_int), ("R", c_int), ("out", c_void_p), ("u", c_void_p)]
+                ("N", c_int), ("G", c_int), ("R", c_int), ("out", c_void_p), ("u", c_void_p),
+                ("scratch", c_void_p)]
 
 
 class LoraGradArgs(ctypes.Structure):
     _fields_ = [("dy", c_void_p), ("x", c_void_p), ("u", c_void_p), ("a", c_void_p), ("b", c_void_p),
                 ("scale", c_void_p), ("rank", c_void_p), ("offsets", c_void_p), ("token_of_row", c_void_p),
                 ("base", c_void_p), ("T", c_int), ("H", c_int), ("N", c_int), ("G", c_int), ("R", c_int),
-                ("dx", c_void_p), ("da", c_void_p), ("db", c_void_p), ("v", c_void_p)]
+                ("dx", c_void_p), ("da", c_void_p), ("db", c_void_p), ("scratch", c_void_p)]
 
 
 LORA_MAX_RANK = 128      # ZMOE_LORA_MAX_RANK

@@ -415,8 +415,10 @@ def lora(x: torch.Tensor, base: Optional[torch.Tensor], a: torch.Tensor, b: torc
     G, R, H, N, pa, pb, ps, pr, po, pt = _adapters(a, b, scale, rank, offsets, token_of_row, T, dev)
     if out is None:
         out = torch.empty(T, N, dtype=_BF16, device=dev)
+    scratch = torch.empty(T, R, dtype=_F32, device=dev)
     args = LoraArgs(_arg(x, "x", _BF16, (T, H), dev), _arg(base, "base", _BF16, (T, N), dev, True), pa, pb, ps, pr,
-                    po, pt, T, H, N, G, R, _arg(out, "out", _BF16, (T, N), dev), _arg(u, "u", _F32, (T, R), dev, True))
+                    po, pt, T, H, N, G, R, _arg(out, "out", _BF16, (T, N), dev), _arg(u, "u", _F32, (T, R), dev, True),
+                    scratch.data_ptr())
     _call(lib.zmoe_lora, args, dev)
     return out
 
@@ -434,10 +436,10 @@ def lora_grad(dy: torch.Tensor, x: torch.Tensor, u: torch.Tensor, a: torch.Tenso
     if dx is None:
         dx = torch.empty(T, H, dtype=_BF16, device=dev)
     da, db = torch.empty_like(a), torch.empty_like(b)
-    v = torch.empty(T, R, dtype=_F32, device=dev)
+    scratch = torch.empty(T, 2 * R, dtype=_F32, device=dev)
     args = LoraGradArgs(_arg(dy, "dy", _BF16, (T, N), dev), _arg(x, "x", _BF16, (T, H), dev),
                         _arg(u, "u", _F32, (T, R), dev), pa, pb, ps, pr, po, pt,
                         _arg(base, "base", _BF16, (T, H), dev, True), T, H, N, G, R,
-                        _arg(dx, "dx", _BF16, (T, H), dev), da.data_ptr(), db.data_ptr(), v.data_ptr())
+                        _arg(dx, "dx", _BF16, (T, H), dev), da.data_ptr(), db.data_ptr(), scratch.data_ptr())
     _call(lib.zmoe_lora_grad, args, dev)
     return dx, da, db
