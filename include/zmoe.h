@@ -306,6 +306,7 @@ zmoe_status zmoe_lora_plan(const int32_t* adapter, int T, int G, int32_t* offset
                            zmoe_stream_t stream);
 
 #define ZMOE_LORA_MAX_RANK 128
+#define ZMOE_LORA_ROWS 512        /* zmoe_lora needs no scratch for up to this many rows */
 
 typedef struct zmoe_lora_args {
   const uint16_t* x;          /* [T, H] BF16 */
@@ -320,7 +321,7 @@ typedef struct zmoe_lora_args {
   uint16_t* out;              /* [T, N] BF16 */
   float* u;                   /* [T, R] fp32 out by row, or NULL: x A^T, kept for zmoe_lora_grad; columns from
                                  the rank on are 0, rows behind the last adapter's are left as they were */
-  float* scratch;             /* [T, R] fp32 */
+  float* scratch;             /* [T, R] fp32; may be NULL when T <= ZMOE_LORA_ROWS */
 } zmoe_lora_args;
 
 zmoe_status zmoe_lora(const zmoe_lora_args* a, zmoe_stream_t stream);

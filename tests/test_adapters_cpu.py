@@ -26,14 +26,14 @@ def _refused(fn, args, text):
 def test_struct_layouts():
     L = _lib()
     names = ["permute_grad", "combine_grad", "lora", "lora_grad"]
-    src = ('#include "zmoe.h"\n#include <stdio.h>\nint main(){printf("%zu %zu %zu %zu %d", '
-           + ", ".join(f"sizeof(zmoe_{n}_args)" for n in names) + ", ZMOE_LORA_MAX_RANK);}")
+    src = ('#include "zmoe.h"\n#include <stdio.h>\nint main(){printf("%zu %zu %zu %zu %d %d", '
+           + ", ".join(f"sizeof(zmoe_{n}_args)" for n in names) + ", ZMOE_LORA_MAX_RANK, ZMOE_LORA_ROWS);}")
     with tempfile.TemporaryDirectory() as d:
         open(os.path.join(d, "s.c"), "w").write(src)
         subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), "-o", os.path.join(d, "s"), os.path.join(d, "s.c")],
                        check=True)
         got = [int(v) for v in subprocess.run([os.path.join(d, "s")], capture_output=True, text=True, check=True).stdout.split()]
-    assert got == [ctypes.sizeof(c) for c in (L.PermuteGradArgs, L.CombineGradArgs, L.LoraArgs, L.LoraGradArgs)] + [L.LORA_MAX_RANK]
+    assert got == [ctypes.sizeof(c) for c in (L.PermuteGradArgs, L.CombineGradArgs, L.LoraArgs, L.LoraGradArgs)] + [L.LORA_MAX_RANK, L.LORA_ROWS]
 
 
 def test_permute_grad_refuses():
@@ -59,7 +59,7 @@ def test_lora_refuses():
     ok = dict(x=P, base=P, a=P, b=P, scale=P, rank=None, offsets=P, token_of_row=None, T=4, H=16, N=16, G=2, R=8, out=P, scratch=P)
     for kw, text in (({"R": 12}, b"R=12"), ({"R": 136}, b"R=136"), ({"R": 0}, b"R=0"), ({"H": 20}, b"H=20"),
                      ({"N": 4}, b"N=4"), ({"G": 0}, b"G < 1"), ({"T": -1}, b"T < 0"), ({"x": None}, b"null"),
-                     ({"offsets": None}, b"null"), ({"scratch": None}, b"null"), ({"a": P + 2}, b"aligned"), ({"out": P + 8}, b"aligned"),
+                     ({"offsets": None}, b"null"), ({"T": 513, "scratch": None}, b"null"), ({"a": P + 2}, b"aligned"), ({"out": P + 8}, b"aligned"),
                      ({"H": 32776}, b"above")):
         _refused(L.lib.zmoe_lora, L.LoraArgs(**dict(ok, **kw)), text)
     ok = dict(dy=P, x=P, u=P, a=P, b=P, scale=P, rank=None, offsets=P, token_of_row=None, base=None, T=4, H=16, N=16,

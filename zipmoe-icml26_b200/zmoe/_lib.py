@@ -84,6 +84,7 @@ class LoraGradArgs(ctypes.Structure):
 
 
 LORA_MAX_RANK = 128      # ZMOE_LORA_MAX_RANK
+LORA_ROWS = 512          # ZMOE_LORA_ROWS
 
 
 class LayerConfig(ctypes.Structure):

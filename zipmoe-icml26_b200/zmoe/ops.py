@@ -19,7 +19,9 @@ ROUTE_QWEN, ROUTE_DEEPSEEK, ROUTE_SWITCH = 0, 1, 2
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """cudaStream_t of torch's current stream on the current device, without
+    building a Stream object (3 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -250,10 +252,8 @@ def permute(topk_idx: torch.Tensor, x: Optional[torch.Tensor], E: int, capacity:
     T, k = topk_idx.shape
     dev = topk_idx.device
     H = x.shape[1] if x is not None else 0
-    counts = torch.empty(E, dtype=torch.int32, device=dev)
-    offsets = torch.empty(E + 1, dtype=torch.int32, device=dev)
-    row_of = torch.empty(T, k, dtype=torch.int32, device=dev)
-    tor = torch.empty(max(T * k, 1), dtype=torch.int32, device=dev)
+    counts, offsets = topk_idx.new_empty(E), topk_idx.new_empty(E + 1)
+    row_of, tor = torch.empty_like(topk_idx), topk_idx.new_empty(max(T * k, 1))
     xp = torch.empty(max(T * k, 1), H, dtype=torch.bfloat16, device=dev) if x is not None else None
     a = PermuteArgs(topk_idx.data_ptr(), _ptr(x), T, H, E, k, capacity, seq_len, counts.data_ptr(),
                     offsets.data_ptr(), row_of.data_ptr(), tor.data_ptr(), _ptr(xp))
@@ -301,31 +301,34 @@ def combine(y: torch.Tensor, row_of: torch.Tensor, topk_w: torch.Tensor, mode: i
 _BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 
 
-def _arg(t: Optional[torch.Tensor], name: str, dtype, shape: tuple, device, optional: bool = False):
+def _arg(t: Optional[torch.Tensor], name: str, dtype, shape: tuple, device: int, optional: bool = False):
     """Device pointer of an argument after checking its type, shape and place."""
     if t is None:
         if not optional:
             raise ValueError(f"{name}: missing")
         return None
-    if t.dtype != dtype or t.device != device or not t.is_contiguous() or tuple(t.shape) != shape:
-        raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {shape} on {device}, "
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {shape} on cuda:{device}, "
                          f"got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _cuda(t: torch.Tensor, name: str, dims: int) -> torch.device:
+def _cuda(t: torch.Tensor, name: str, dims: int) -> int:
+    """Device index of a CUDA tensor with `dims` dimensions."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != dims:
         raise ValueError(f"{name}: expected a CUDA tensor with {dims} dimensions")
-    return t.device
+    return t.get_device()
 
 
-def _call(fn, args, device):
+def _call(fn, args, device: int):
     """Runs an entry point on the arguments' device and that device's current stream."""
-    if device.index == torch.cuda.current_device():
-        check(fn(ctypes.byref(args), _stream()), fn.__name__)
+    if device == torch._C._cuda_getDevice():
+        status = fn(ctypes.byref(args), _stream())
     else:
         with torch.cuda.device(device):
-            check(fn(ctypes.byref(args), _stream()), fn.__name__)
+            status = fn(ctypes.byref(args), _stream())
+    if status:
+        check(status, fn.__name__)
 
 
 def permute_grad(dxp: torch.Tensor, row_of: torch.Tensor, base: Optional[torch.Tensor] = None,
@@ -337,7 +340,7 @@ def permute_grad(dxp: torch.Tensor, row_of: torch.Tensor, base: Optional[torch.T
     _cuda(row_of, "row_of", 2)
     T, k = row_of.shape
     if dx is None:
-        dx = torch.empty(T, H, dtype=_BF16, device=dev)
+        dx = dxp.new_empty(T, H)
     a = PermuteGradArgs(_arg(dxp, "dxp", _BF16, (rows, H), dev), _arg(row_of, "row_of", _I32, (T, k), dev),
                         _arg(base, "base", _BF16, (T, H), dev, True), T, H, k, rows,
                         _arg(dx, "dx", _BF16, (T, H), dev))
@@ -361,11 +364,11 @@ def combine_grad(dout: torch.Tensor, y: torch.Tensor, row_of: torch.Tensor, topk
     if shared_gate is not None and y_shared is None:
         raise ValueError("shared_gate without y_shared")
     if dy is None:
-        dy = torch.empty(rows, H, dtype=_BF16, device=dev)
-    dw = torch.empty(T, k, dtype=_F32, device=dev)
-    dysh = torch.empty(T, H, dtype=_BF16, device=dev) if y_shared is not None else None
-    dg = torch.empty(T, dtype=_F32, device=dev) if shared_gate is not None else None
-    dx = torch.empty(T, H, dtype=_BF16, device=dev) if mode == ROUTE_SWITCH else None
+        dy = torch.empty_like(y)
+    dw = topk_w.new_empty(T, k)
+    dysh = torch.empty_like(dout) if y_shared is not None else None
+    dg = topk_w.new_empty(T) if shared_gate is not None else None
+    dx = torch.empty_like(dout) if mode == ROUTE_SWITCH else None
     a = CombineGradArgs(_arg(dout, "dout", _BF16, (T, H), dev), _arg(y, "y", _BF16, (rows, H), dev),
                         _arg(y_shared, "y_shared", _BF16, (T, H), dev, True),
                         _arg(shared_gate, "shared_gate", _F32, (T,), dev, True),
@@ -382,8 +385,7 @@ def lora_plan(adapter: torch.Tensor, G: int):
     token_of_row [T], which serve every projection of the step."""
     dev = _cuda(adapter, "adapter", 1)
     T = adapter.shape[0]
-    offsets = torch.empty(max(G, 0) + 1, dtype=_I32, device=dev)
-    tor = torch.empty(T, dtype=_I32, device=dev)
+    offsets, tor = adapter.new_empty(max(G, 0) + 1), adapter.new_empty(T)
     ids = _arg(adapter, "adapter", _I32, (T,), dev)
     with torch.cuda.device(dev):
         check(lib.zmoe_lora_plan(ids, T, G, offsets.data_ptr(), tor.data_ptr(), _stream()), "zmoe_lora_plan")
@@ -414,11 +416,11 @@ def lora(x: torch.Tensor, base: Optional[torch.Tensor], a: torch.Tensor, b: torc
     T = x.shape[0]
     G, R, H, N, pa, pb, ps, pr, po, pt = _adapters(a, b, scale, rank, offsets, token_of_row, T, dev)
     if out is None:
-        out = torch.empty(T, N, dtype=_BF16, device=dev)
-    scratch = torch.empty(T, R, dtype=_F32, device=dev)
+        out = x.new_empty(T, N)
+    scratch = x.new_empty(T, 2 * R) if T > _lib.LORA_ROWS else None
     args = LoraArgs(_arg(x, "x", _BF16, (T, H), dev), _arg(base, "base", _BF16, (T, N), dev, True), pa, pb, ps, pr,
                     po, pt, T, H, N, G, R, _arg(out, "out", _BF16, (T, N), dev), _arg(u, "u", _F32, (T, R), dev, True),
-                    scratch.data_ptr())
+                    _ptr(scratch))
     _call(lib.zmoe_lora, args, dev)
     return out
 
@@ -434,9 +436,9 @@ def lora_grad(dy: torch.Tensor, x: torch.Tensor, u: torch.Tensor, a: torch.Tenso
     T = dy.shape[0]
     G, R, H, N, pa, pb, ps, pr, po, pt = _adapters(a, b, scale, rank, offsets, token_of_row, T, dev)
     if dx is None:
-        dx = torch.empty(T, H, dtype=_BF16, device=dev)
+        dx = dy.new_empty(T, H)
     da, db = torch.empty_like(a), torch.empty_like(b)
-    scratch = torch.empty(T, 2 * R, dtype=_F32, device=dev)
+    scratch = dy.new_empty(T, 4 * R)
     args = LoraGradArgs(_arg(dy, "dy", _BF16, (T, N), dev), _arg(x, "x", _BF16, (T, H), dev),
                         _arg(u, "u", _F32, (T, R), dev), pa, pb, ps, pr, po, pt,
                         _arg(base, "base", _BF16, (T, H), dev, True), T, H, N, G, R,
