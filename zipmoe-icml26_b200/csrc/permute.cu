@@ -139,9 +139,10 @@ scatter_kernel(const int32_t* __restrict__ topk_idx, int T, int k, int E,
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortE = 1024;          // experts: one per thread in the scan, 128 KB of warp counts
-constexpr int kSortCluster = 8;
+constexpr int kSortCluster = 16;      // the steps are bound by instruction issue: 98 thousand
+                                      // pairs took 19 us on 8 SMs, 12 on 16
 constexpr int kFusedPairs = 2048;     // pairs every CTA of the fused launch sorts for itself
-constexpr int kBatch = 4;             // steps whose loads are issued together
+constexpr int kHold = 16;             // steps of a warp whose pairs stay in registers between the two walks
 constexpr unsigned kFull = 0xffffffffu;
 
 struct SortArgs {
@@ -151,7 +152,7 @@ struct SortArgs {
   int32_t* counts;                    // [E] or nullptr
   int32_t* offsets;                   // [E + 1]; with rest the first E entries
   int32_t* row_of;                    // [T, k] or nullptr
-  int32_t* token_of_row;              // [T * k]
+  int32_t* token_of_row;              // [T * k] or nullptr: the copy of the rows writes it
 };
 
 // Sorts the pairs of tokens [0, T) by expert over the CTAs of a cluster (rank
@@ -178,7 +179,8 @@ __device__ void sort_pairs(const SortArgs& a, int rank, int csize, int* smem, bo
   for (int e = lane; e < E; e += 32) my[e] = 0;
   __syncwarp();
 
-  // one step: the expert of this lane's pair (-1: no row) and the lanes that share it
+  // A step's pair of this lane as seen by the warp: expert, earlier lanes with
+  // the same expert << 10, lanes with it << 16; -1: no row, -2: no pair.
   auto load = [&](int s) -> int {
     const int t = s * tp + tl;
     if (!used || s >= s1 || t >= a.T) return -2;
@@ -186,22 +188,42 @@ __device__ void sort_pairs(const SortArgs& a, int rank, int csize, int* smem, bo
     if (a.rest) return (unsigned)e < (unsigned)(E - 1) ? e : E - 1;
     return (unsigned)e < (unsigned)E ? e : -1;
   };
-  auto peers = [&](int& e) -> unsigned {
-    unsigned m = __match_any_sync(kFull, e);
+  auto pack = [&](int e) -> int {
+    // lanes with the same expert: one vote per bit of it (a match.any instead
+    // took 0.4 us more per step of an SM's warps)
+    unsigned m = __ballot_sync(kFull, e >= 0);
+#pragma unroll
+    for (int b = 0; b < 10; ++b) {
+      if (E <= 1 << b) break;
+      const unsigned v = __ballot_sync(kFull, e >> b & 1);
+      m &= e >> b & 1 ? v : ~v;
+    }
     if (e >= 0 && (m & earlier)) e = -1;               // an expert named twice by a token counts once
-    return m & __ballot_sync(kFull, e >= 0);
+    m &= __ballot_sync(kFull, e >= 0);
+    return e < 0 ? e : e | __popc(m & ((1u << lane) - 1u)) << 10 | __popc(m) << 16;
+  };
+  auto count = [&](int v) {                            // the first lane of an expert adds for all
+    if (v >= 0 && !(v >> 10 & 63)) my[v & 1023] += v >> 16;
+    __syncwarp();
   };
 
-  for (int s = s0; s < s1; s += kBatch) {
-    int ev[kBatch];
+  int held[kHold];
+  const bool hold = per <= kHold;
+  if (hold) {
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) ev[b] = load(s + b);
+    for (int b = 0; b < kHold; ++b) held[b] = load(s0 + b);
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      int e = ev[b];
-      const unsigned m = peers(e);
-      if (e >= 0 && lane == __ffs(m) - 1) my[e] += __popc(m);
-      __syncwarp();
+    for (int b = 0; b < kHold; ++b) {
+      if (b >= per) break;
+      held[b] = pack(held[b]);
+      count(held[b]);
+    }
+  } else {
+    for (int s = s0; s < s1; s += kHold) {
+#pragma unroll
+      for (int b = 0; b < kHold; ++b) held[b] = load(s + b);
+#pragma unroll
+      for (int b = 0; b < kHold; ++b) count(pack(held[b]));
     }
   }
   __syncthreads();
@@ -221,10 +243,13 @@ __device__ void sort_pairs(const SortArgs& a, int rank, int csize, int* smem, bo
   const int e1 = threadIdx.x;
   if (e1 < E) {
     if (csize > 1) {
-      for (int c = 0; c < csize; ++c) {
-        const int n = *cg::this_cluster().map_shared_rank(tot + e1, c);
-        if (c < rank) before += n;
-        all += n;
+      int n[kSortCluster];
+#pragma unroll
+      for (int c = 0; c < kSortCluster; ++c) n[c] = *cg::this_cluster().map_shared_rank(tot + e1, c);
+#pragma unroll
+      for (int c = 0; c < kSortCluster; ++c) {
+        if (c < rank) before += n[c];
+        all += n[c];
       }
     } else {
       all = tot[e1];
@@ -259,28 +284,31 @@ __device__ void sort_pairs(const SortArgs& a, int rank, int csize, int* smem, bo
   }
   __syncthreads();
 
-  for (int s = s0; s < s1; s += kBatch) {
-    int ev[kBatch];
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) ev[b] = load(s + b);
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      int e = ev[b];
-      const bool pair = e >= -1;
-      const unsigned m = peers(e);
-      const int t = (s + b) * tp + tl;
-      int row = -1;
-      if (e >= 0) row = base[e] + my[e] + __popc(m & ((1u << lane) - 1u));
-      __syncwarp();
-      if (e >= 0 && lane == __ffs(m) - 1) my[e] += __popc(m);
-      __syncwarp();
-      if (pair) {
-        if (rows_s) rows_s[t * k + jl] = row;
-        if (write) {
-          if (a.row_of) a.row_of[(size_t)t * k + jl] = row;
-          if (row >= 0) a.token_of_row[row] = t;
-        }
+  auto place = [&](int s, int v) {
+    const int t = s * tp + tl;
+    const int row = v >= 0 ? base[v & 1023] + my[v & 1023] + (v >> 10 & 63) : -1;
+    __syncwarp();
+    count(v);
+    if (v >= -1) {
+      if (rows_s) rows_s[t * k + jl] = row;
+      if (write) {
+        if (a.row_of) a.row_of[(size_t)t * k + jl] = row;
+        if (a.token_of_row && row >= 0) a.token_of_row[row] = t;
       }
+    }
+  };
+  if (hold) {
+#pragma unroll
+    for (int b = 0; b < kHold; ++b) {
+      if (b >= per) break;
+      place(s0 + b, held[b]);
+    }
+  } else {
+    for (int s = s0; s < s1; s += kHold) {
+#pragma unroll
+      for (int b = 0; b < kHold; ++b) held[b] = load(s + b);
+#pragma unroll
+      for (int b = 0; b < kHold; ++b) place(s + b, pack(held[b]));
     }
   }
 }
@@ -316,11 +344,13 @@ sort_gather_kernel(const SortArgs a, const uint4* __restrict__ x, int vec, uint4
   }
 }
 
-// xp[row_of[t, j]] = x[t] for every slot j with a row.  A dependent launch: x
+// xp[row_of[t, j]] = x[t] and token_of_row[row_of[t, j]] = t for every slot j with
+// a row (the latter is one 4-byte store per row wherever it lands: a cluster's
+// few SMs took 6 us for 98 thousand, here they ride along).  A dependent launch: x
 // was complete before the sort began, so its loads do not wait for the sort.
 __global__ void __launch_bounds__(kThreads)
 scatter_rows_kernel(const uint4* __restrict__ x, int T, int vec, int k, const int32_t* __restrict__ row_of,
-                    uint4* __restrict__ xp, int max_rows) {
+                    uint4* __restrict__ xp, int max_rows, int32_t* __restrict__ token_of_row) {
   const size_t first = (size_t)blockIdx.x * kThreads;
   const unsigned rem = (unsigned)(first % vec) + threadIdx.x;
   const size_t t = first / vec + rem / vec;
@@ -331,7 +361,10 @@ scatter_rows_kernel(const uint4* __restrict__ x, int T, int vec, int k, const in
   if (t >= (size_t)T) return;
   for (int j = 0; j < k; ++j) {
     const int r = row_of[t * k + j];
-    if ((unsigned)r < (unsigned)max_rows) __stcs(xp + (size_t)r * vec + c, v);
+    if ((unsigned)r < (unsigned)max_rows) {
+      __stcs(xp + (size_t)r * vec + c, v);
+      if (c == 0 && token_of_row) token_of_row[r] = (int)t;
+    }
   }
 }
 
@@ -348,15 +381,22 @@ gather_rows_kernel(const uint4* __restrict__ src, const int32_t* __restrict__ in
   }
 }
 
-// One cluster: a single CTA while its 32 warps have at most four batches of
-// steps each, else the largest portable size.
+// One cluster: a single CTA while its warps hold their pairs, else the largest
+// size.
 zmoe_status launch_sort(const SortArgs& a, cudaStream_t stream) {
   const size_t smem = sort_smem(a.E);
   zmoe_status st = allow_smem<sort_kernel>();
   if (st != ZMOE_OK) return st;
+  static std::atomic<uint64_t> wide{0};                // devices on which the kernel may use 16-CTA clusters
+  int dev = 0;
+  ZMOE_CUDA_RET(cudaGetDevice(&dev));
+  if (!(wide.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
+    ZMOE_CUDA_RET(cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    wide.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
+  }
   const int tp = 32 / a.k, steps = (a.T + tp - 1) / tp;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(steps <= 4 * kBatch * kSortWarps ? 1 : kSortCluster);
+  cfg.gridDim = dim3(steps <= kHold * kSortWarps ? 1 : kSortCluster);
   cfg.blockDim = dim3(kSortThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -388,8 +428,9 @@ zmoe_status launch_permute(const zmoe_permute_args* a, cudaStream_t stream) {
   ZMOE_CHECK_ARG((long long)a->T * a->k < (1LL << 31), "permute: T=%d x k=%d pairs are too many", a->T, a->k);
   const int vec = a->H / 8;
   zmoe_status st;
+  bool copies_tokens = false;
   if (a->capacity <= 0 && a->E <= kSortE && a->k <= 32) {
-    const SortArgs sa{a->topk_idx, a->T, a->k, a->E, 0, a->counts, a->offsets, a->row_of, a->token_of_row};
+    SortArgs sa{a->topk_idx, a->T, a->k, a->E, 0, a->counts, a->offsets, a->row_of, a->token_of_row};
     if (a->xp && a->T * a->k <= kFusedPairs && vec > 0) {
       st = allow_smem<sort_gather_kernel>();
       if (st != ZMOE_OK) return st;
@@ -400,7 +441,9 @@ zmoe_status launch_permute(const zmoe_permute_args* a, cudaStream_t stream) {
                                                                  reinterpret_cast<uint4*>(a->xp));
       return launch_status("sort_gather_kernel");
     }
+    if (a->xp && vec > 0) sa.token_of_row = nullptr;
     st = launch_sort(sa, stream);
+    copies_tokens = true;
   } else {
     ZMOE_CUDA_RET(cudaMemsetAsync(a->row_of, 0xff, sizeof(int32_t) * (size_t)a->T * a->k, stream));
     count_kernel<<<a->E, kThreads, 0, stream>>>(a->topk_idx, a->T, a->k, a->capacity, a->seq_len, a->counts);
@@ -423,7 +466,8 @@ zmoe_status launch_permute(const zmoe_permute_args* a, cudaStream_t stream) {
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   ZMOE_CUDA_RET(cudaLaunchKernelEx(&cfg, scatter_rows_kernel, reinterpret_cast<const uint4*>(a->x), a->T, vec, a->k,
-                                   (const int32_t*)a->row_of, reinterpret_cast<uint4*>(a->xp), a->T * a->k));
+                                   (const int32_t*)a->row_of, reinterpret_cast<uint4*>(a->xp), a->T * a->k,
+                                   copies_tokens ? a->token_of_row : (int32_t*)nullptr));
   return launch_status("scatter_rows_kernel");
 }
 
