@@ -11,7 +11,7 @@
 //                       share of the output columns).  Launched as a dependent of
 //                       the shrink: it loads base and weights while that ends.
 //   lora_dw_kernel      dA^T = x^T v and dB = s dy^T u: the rows of an adapter as
-//                       the contraction, one tile of 128 columns of x or dy per
+//                       the contraction, one tile of 256 columns of x or dy per
 //                       cluster, whose CTAs share the rows.
 // (A single kernel for shrink and expand, with u kept in TMEM, measured slower:
 // 31.5 against 29 us for 8191 rows of 2048 in and out at rank 64, 40 against 20 us
@@ -84,6 +84,7 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
+__device__ __forceinline__ void prefetch(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // The MMA warp runs its loop with all lanes, so that barrier addresses and
@@ -344,6 +345,14 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), csize = (int)cl.num_blocks();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // the token list, a share a CTA, and the ranks and scales come to L2 while the
+  // unit is looked for, instead of one after the other behind it
+  if (a.token_of_row)
+    for (int i = 32 * (blockIdx.x * L::kThreads + tid); i < a.T; i += 32 * gridDim.x * L::kThreads) prefetch(a.token_of_row + i);
+  if (32 * tid < a.G) {
+    if (a.rank) prefetch(a.rank + 32 * tid);
+    if (a.scale) prefetch(a.scale + 32 * tid);
+  }
   if (warp == 0) {
     const Unit u = find_unit(a.offsets, a.G, a.T, kTile, false, (int)((gridDim.x - 1 - blockIdx.x) / csize));
     if (lane == 0) unit_s = u;
@@ -407,7 +416,6 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
 #pragma unroll
       for (int e = 0; e < kTurn; ++e) at.next();
     }
-    wait_bar(smem_u32(&sums), 0, &failed);             // every MMA has read the ring
   } else {
     // ------------------------------------------------------------------ MMAs
     // Its instructions are the step's critical path: descriptors are built once
@@ -435,8 +443,14 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
   float4* part = reinterpret_cast<float4*>(smem);      // [rp / 4][kTile][4], in the ring's place
   const bool mine = m < un.rows && warp < kMmaWarp;
   const size_t grow = (size_t)(un.row0 + m);
-  tc_fence_after();
-  auto write = [&](int i, float (&f)[8]) {
+  auto load_u = [&](int i, float4 (&u)[2]) {           // the forward pass's u at this row's columns 8 i on
+    if (DIR == 1 && a.u_in && mine && 8 * i < min(rp, R)) {
+      const float4* up = reinterpret_cast<const float4*>(a.u_in + grow * R + 8 * i);
+      u[0] = __ldg(up);
+      u[1] = __ldg(up + 1);
+    }
+  };
+  auto write = [&](int i, float (&f)[8], const float4 (&u)[2]) {
     const int c0 = 8 * i;
     if (!mine || c0 >= R) return;
 #pragma unroll
@@ -455,9 +469,7 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
     *reinterpret_cast<uint4*>(sp) = hi;
     *reinterpret_cast<uint4*>(sp + R) = lo;
     if (DIR == 1 && a.u_in) {
-      const float4* up = reinterpret_cast<const float4*>(a.u_in + grow * R + c0);
-      const float4 u0 = __ldg(up), u1 = __ldg(up + 1);
-      float w[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
+      float w[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (c0 + e >= rk) w[e] = 0.0f;
@@ -466,12 +478,20 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
       *reinterpret_cast<uint4*>(sp + 3 * R) = lo;
     }
   };
+  const int first = csize == 1 ? half : rank + csize * half, stride = 2 * csize;
+  float4 u[2];
+  if (warp < kMmaWarp) {
+    load_u(first, u);
+    wait_bar(smem_u32(&sums), 0, &failed);             // every MMA has read the ring
+  }
+  tc_fence_after();
   if (csize == 1) {
     if (warp < kMmaWarp)
-      for (int i = half; i < n8; i += 2) {
+      for (int i = first; i < n8; i += stride) {
         float f[8];
         tmem_ld8(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(8 * i), f);
-        write(i, f);
+        if (i != first) load_u(i, u);
+        write(i, f, u);
       }
   } else {
     if (warp < kMmaWarp)
@@ -483,7 +503,7 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
       }
     cl.sync();
     if (warp < kMmaWarp)
-      for (int i = rank + csize * half; i < n8; i += 2 * csize) {
+      for (int i = first; i < n8; i += stride) {
         float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         for (int cc = 0; cc < csize; cc += 4) {        // four CTAs' loads in flight, added in rank order
           float4 v[4][2];
@@ -502,9 +522,10 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
             f[4] += v[c][1].x; f[5] += v[c][1].y; f[6] += v[c][1].z; f[7] += v[c][1].w;
           }
         }
-        write(i, f);
+        if (i != first) load_u(i, u);
+        write(i, f, u);
       }
-    cl.sync();                                         // partial sums stay until every CTA has read them
+    cl.barrier_arrive();                               // partial sums stay until every CTA has read them
   }
   if (DIR == 0 && a.u && rank == 0 && mine && half == 0)
     for (int c = rp; c < R; c += 4) *reinterpret_cast<float4*>(a.u + grow * R + c) = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -512,6 +533,7 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
   __syncthreads();
   tc_fence_after();
   free_tmem();
+  if (csize > 1) cl.barrier_wait();
 }
 
 // ---------------------------------------------------------------------------
@@ -745,14 +767,19 @@ struct DwArgs {
   int T, G, R;
 };
 
-// A step is 32 rows: 8 KB of x or dy and RB x 8 KB of the factor's two halves.
+// A step is 32 rows of 256 columns: 16 KB of x or dy and RB x 8 KB of the
+// factor's two halves.  (With 128 columns the factor is read twice as often and
+// there are twice as many CTAs to set up: 40 against 30 us for 60 groups of
+// 273 rows, 2048 and 1408 columns, rank 32.)
 template <int RB>
 struct Dw {
-  static constexpr int kRows = 32;
-  static constexpr uint32_t kSrcBytes = kRows * kTile * 2, kHalf = RB * kRows * 128;
+  static constexpr int kRows = 32, kCols = 2 * kTile;
+  static constexpr uint32_t kBlock = kRows * 128;      // 64 columns
+  static constexpr uint32_t kSrcBytes = kRows * kCols * 2, kHalf = RB * kBlock;
   static constexpr uint32_t kStageBytes = kSrcBytes + 2 * kHalf;
-  static constexpr int kPerSM = RB == 1 ? 4 : 2;
-  static constexpr int kStages = RB == 1 ? 3 : 4;      // 48 KB / 96 KB
+  static constexpr int kPerSM = RB == 1 ? 2 : 1;
+  static constexpr int kStages = RB == 1 ? 4 : 6;      // 96 KB / 192 KB
+  static constexpr uint32_t kTmemCols = 2 * RB * 64;
   static constexpr int kSmem = 1024 + kStages * kStageBytes;
 };
 
@@ -769,16 +796,16 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), csize = (int)cl.num_blocks();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int tilesA = (a.M[0] + kTile - 1) / kTile;
+  const int tilesA = (a.M[0] + D::kCols - 1) / D::kCols;
   const int unit = (int)(blockIdx.x / csize), g = blockIdx.y;
-  const int which = unit >= tilesA, m0 = (which ? unit - tilesA : unit) * kTile, M = a.M[which];
+  const int which = unit >= tilesA, m0 = (which ? unit - tilesA : unit) * D::kCols, M = a.M[which];
   const int R = a.R, rk = rank_of(a.rank, g, R);
   const int r0 = min(max(a.offsets[g], 0), a.T), r1 = min(max(a.offsets[g + 1], 0), a.T);
   uint16_t* out = a.out[which];
-  const int m = m0 + tid;                              // a drain thread's column of src (TMEM lane)
 
-  // eight rank columns from c0 on of column m
-  auto store = [&](int c0, const float (&v)[8]) {
+  // eight rank columns from c0 on of column m0 + tid (TMEM lane) + 128 t
+  auto store = [&](int t, int c0, const float (&v)[8]) {
+    const int m = m0 + t * kTile + tid;
     if (tid >= kTile || m >= M || c0 >= R) return;
     if (which) {
       *reinterpret_cast<uint4*>(out + ((size_t)g * M + m) * R + c0) =
@@ -790,7 +817,10 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
   };
   const float zero8[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   const int rp = r1 > r0 ? (rk + 15) & ~15 : 0;
-  for (int c = rp / 8 + rank; c < R / 8; c += csize) store(8 * c, zero8);
+  for (int c = rp / 8 + rank; c < R / 8; c += csize) {
+    store(0, 8 * c, zero8);
+    store(1, 8 * c, zero8);
+  }
   if (rp == 0) {                                       // the whole cluster leaves
     // but the launch does not end before the one that it depends on
     if (blockIdx.x == 0 && blockIdx.y == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -813,7 +843,7 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
   }
   if (warp == kLoadWarps) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
-                 "r"(128)
+                 "r"(D::kTmemCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -827,7 +857,7 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
     {
       const uint32_t go = elect_one();
       const uint32_t id = idesc(rp, 1, 1);
-      const uint64_t dx0 = desc_mn(ring, kRows * 128), dw0 = desc_mn(ring + D::kSrcBytes, kRows * 128);
+      const uint64_t dx0 = desc_mn(ring, D::kBlock), dw0 = desc_mn(ring + D::kSrcBytes, D::kBlock);
       Ring<kStages> at;
 #pragma unroll 1
       for (int s = 0; s < ns; ++s) {
@@ -836,9 +866,13 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
         const uint32_t off = at.slot * (D::kStageBytes >> 4);
 #pragma unroll
         for (int kk = 0; kk < kRows / 16; ++kk) {
-          const uint64_t da = dx0 + off + kk * (2048 >> 4), dw = dw0 + off + kk * (2048 >> 4);
-          mma_ss(tmem, da, dw, id, (s | kk) != 0, go);
-          mma_ss(tmem, da, dw + (D::kHalf >> 4), id, 1, go);
+          const uint64_t dw = dw0 + off + kk * (2048 >> 4);
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const uint64_t da = dx0 + off + kk * (2048 >> 4) + n * (2 * D::kBlock >> 4);
+            mma_ss(tmem + n * RB * 64, da, dw, id, (s | kk) != 0, go);
+            mma_ss(tmem + n * RB * 64, da, dw + (D::kHalf >> 4), id, 1, go);
+          }
         }
         commit_at(used_a + 8 * at.slot, go);
         at.next();
@@ -848,12 +882,12 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
     __syncwarp();
   } else {
     // ------------------------------------------------------------------ loaders
-    // 32 rows x 128 columns of src per step: this thread's chunk of rows
-    // tid/16 + 8j; the factor's two halves: rows tid/8 + 16j, chunk tid%8 (+ 8)
-    const int ch = tid & 15, col = m0 + 8 * ch, xr = tid >> 4, fr = tid >> 3, fc = tid & 7;
+    // 32 rows x 256 columns of src per step: this thread's chunk (its lane) of rows
+    // warp + 4j; the factor's two halves: rows tid/8 + 16j, chunk tid%8 (+ 8)
+    const int col = m0 + 8 * lane, fr = tid >> 3, fc = tid & 7;
     uint32_t xo[2], fo = D::kSrcBytes + place(fr, fc, 0);
-    xo[0] = place(xr, ch, kRows * 128);                // + 2048 for rows 16 on
-    xo[1] = place(xr + 8, ch, kRows * 128);
+    xo[0] = place(warp, lane, D::kBlock);              // + 1024 every eight rows
+    xo[1] = place(warp + 4, lane, D::kBlock);
     const uint16_t* src = a.src[which];
     const int n8 = min(rp, R) / 8;                     // chunks in memory; zeros behind them up to rp / 8
     const uint16_t* fp = a.split + ((size_t)(r0 + sb * kRows + fr) * 4 + 2 * which) * R + 8 * fc;
@@ -882,10 +916,10 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
         const uint32_t st = ring + at.slot * D::kStageBytes;
         const int row = first + s * kRows;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int t = __shfl_sync(kFull, cur[e], xr + 8 * j);
+        for (int j = 0; j < kRows / 4; ++j) {
+          const int t = __shfl_sync(kFull, cur[e], warp + 4 * j);
           const bool in = (unsigned)t < (unsigned)a.T;
-          cp16(st + xo[j & 1] + 2048u * (j >> 1), in ? xsrc + (size_t)(unsigned)t * (unsigned)M : src, in ? xbytes : 0);
+          cp16(st + xo[j & 1] + 1024u * (j >> 1), in ? xsrc + (size_t)(unsigned)t * (unsigned)M : src, in ? xbytes : 0);
         }
 #pragma unroll
         for (int i = 0; i < RB; ++i) {
@@ -912,26 +946,29 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
     tc_fence_after();
   }
   __syncthreads();                                     // the ring is free: partial sums take its place
-  float4* part = reinterpret_cast<float4*>(smem);      // [rp / 4][kTile][4]
+  float4* part = reinterpret_cast<float4*>(smem);      // [2][rp / 4][kTile][4]
   const float scale = which && a.scale ? a.scale[g] : 1.0f;
+  const int n8 = rp / 8;
   if (warp < kLoadWarps) {
-    for (int c = 0; c < rp / 8; ++c) {
+    for (int c = 0; c < 2 * n8; ++c) {                 // tile c / n8, rank columns 8 (c % n8) on
+      const int t = c >= n8, c8 = 8 * (c - t * n8);
       float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (ns > 0) tmem_ld8(tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(8 * c), v);
+      if (ns > 0) tmem_ld8(tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(t * RB * 64 + c8), v);
       if (csize > 1) {
         part[(2 * c) * kTile + tid] = make_float4(v[0], v[1], v[2], v[3]);
         part[(2 * c + 1) * kTile + tid] = make_float4(v[4], v[5], v[6], v[7]);
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = 8 * c + e < rk ? v[e] * scale : 0.0f;
-        store(8 * c, v);
+        for (int e = 0; e < 8; ++e) v[e] = c8 + e < rk ? v[e] * scale : 0.0f;
+        store(t, c8, v);
       }
     }
   }
   if (csize > 1) {
     cl.sync();
     if (warp < kLoadWarps) {
-      for (int c = rank; c < rp / 8; c += csize) {
+      for (int c = rank; c < 2 * n8; c += csize) {
+        const int t = c >= n8, c8 = 8 * (c - t * n8);
         float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         for (int pc = 0; pc < csize; pc += 4) {        // four CTAs' loads in flight, added in rank order
           float4 w[4][2];
@@ -951,8 +988,8 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
           }
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = 8 * c + e < rk ? v[e] * scale : 0.0f;
-        store(8 * c, v);
+        for (int e = 0; e < 8; ++e) v[e] = c8 + e < rk ? v[e] * scale : 0.0f;
+        store(t, c8, v);
       }
     }
     cl.sync();                                         // partial sums stay until every CTA has read them
@@ -961,7 +998,7 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
   __syncthreads();
   if (warp == kLoadWarps) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(128) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(D::kTmemCols) : "memory");
   }
 }
 
@@ -1024,9 +1061,10 @@ zmoe_status launch_tiles(TileArgs a, cudaStream_t stream) {
 
 template <int RB>
 zmoe_status launch_dw(const DwArgs& a, cudaStream_t stream) {
+  using D = Dw<RB>;
   zmoe_status st = allow_smem<lora_dw_kernel<RB>>();
   if (st != ZMOE_OK) return st;
-  const int tiles = (a.M[0] + kTile - 1) / kTile + (a.M[1] + kTile - 1) / kTile;
+  const int tiles = (a.M[0] + D::kCols - 1) / D::kCols + (a.M[1] + D::kCols - 1) / D::kCols;
   const int steps = (a.T + Dw<RB>::kRows - 1) / Dw<RB>::kRows;
   const int csize = share((long long)tiles * a.G, (steps + a.G - 1) / a.G, kNumSMs * Dw<RB>::kPerSM, 2, 8, 8, true);
   return launch(lora_dw_kernel<RB>, dim3((unsigned)(tiles * csize), (unsigned)a.G), kDwThreads, csize, true,
