@@ -61,9 +61,9 @@ const char* zmoe_last_error(void);
  * No counterpart in the reference, whose libtorch FFN has no device waits. */
 zmoe_status zmoe_kernel_error(int32_t* code, int reset);
 /* Test hook for the error path above (no counterpart in the reference): later
- * expert-FFN launches from this process use wait_cycles (clock64 cycles; <= 0
+ * expert-FFN and adapter launches from this process use wait_cycles (clock64 cycles; <= 0
  * restores the default of about 2 s) as their wait limit, and with
- * drop_loads != 0 their TMA producer issues no loads, so that the first MMA
+ * drop_loads != 0 their producers issue no loads, so that the first MMA
  * wait runs out and the launch returns through the error path.  Nothing
  * faults or hangs: every wait stays bounded. */
 zmoe_status zmoe_debug_ffn_wait(long long wait_cycles, int drop_loads);
@@ -295,8 +295,8 @@ zmoe_status zmoe_combine_grad(const zmoe_combine_grad_args* a, zmoe_stream_t str
  * with base = the shared projection's output.  Rows are grouped by adapter:
  * rows offsets[g] .. offsets[g + 1] belong to adapter g, row r is token
  * token_of_row[r] (NULL: row r is token r, as for zmoe_permute's gathered
- * rows with an adapter per expert).  Rows from offsets[G] to T use no adapter:
- * out = base.  rank[g] <= R is the rank of adapter g: rows of A_g and columns
+ * rows with an adapter per expert).  Rows outside [offsets[0], offsets[G]) use no
+ * adapter: out = base.  rank[g] <= R is the rank of adapter g: rows of A_g and columns
  * of B_g from rank[g] on are not used, whatever they hold.
  * ------------------------------------------------------------------------ */
 /* Rows of a batch from each token's adapter id: offsets [G + 1] and

@@ -56,6 +56,9 @@ constexpr long long kWaitCycles = 4000000000LL;   // about 2 s at 1.9 GHz
 long long g_wait_limit = kWaitCycles;
 int g_drop_loads = 0;
 
+long long wait_limit() { return g_wait_limit; }
+int drop_loads() { return g_drop_loads; }
+
 struct __align__(64) Params {
   CUtensorMap amap[kMaxMaps];         // weight (A) maps: MODE 0 uses 2 per group
   CUtensorMap bmap;                   // activation (B) map over [rows_total, K]

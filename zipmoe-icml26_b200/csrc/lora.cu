@@ -251,7 +251,7 @@ zmoe_status launch_lora(const zmoe_lora_args* a, cudaStream_t stream) {
   if (a->T > 2 * ZMOE_LORA_ROWS || (a->T > ZMOE_LORA_ROWS && a->R > 32 && a->G < 32)) return launch_tiles(a, stream);
   // as many CTAs per unit as fit the SMs together, two on each
   const int about = (a->T + kRows - 1) / kRows + (a->T < a->G ? a->T : a->G) / 2;
-  const int units = a->T / kRows + (a->T < a->G + 1 ? a->T : a->G + 1);
+  const int units = a->T / kRows + (a->T < a->G + 2 ? a->T : a->G + 2);
   int csize = kCluster;
   while (csize > 1 && about * csize > 2 * kNumSMs) csize /= 2;
   cudaLaunchConfig_t cfg{};

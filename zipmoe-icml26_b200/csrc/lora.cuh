@@ -15,17 +15,17 @@ zmoe_status launch_tiles(const zmoe_lora_args* a, cudaStream_t stream);
 zmoe_status launch_grad_tiles(const zmoe_lora_grad_args* a, cudaStream_t stream);
 zmoe_status read_error(int32_t* out, int reset);
 
-// Up to `tile` consecutive rows of one group; g == G: the rows without adapter.
+// Up to `tile` consecutive rows of one group; g >= G: rows without adapter.
 struct Unit {
   int g, row0, rows;                                   // rows == 0: no such unit
 };
 
 // Unit u of the groups' tiles, in order; `rest`: the rows behind the last
-// group are a group too.  Called by one full warp; offsets are clamped to
+// group, and those before the first, are groups too.  Called by one full warp; offsets are clamped to
 // [0, T], so a unit never reaches past the last row.
 __device__ __forceinline__ Unit find_unit(const int32_t* __restrict__ offsets, int G, int T, int tile, bool rest, int u) {
   const int lane = threadIdx.x & 31;
-  const int groups = G + (rest ? 1 : 0);
+  const int groups = G + (rest ? 2 : 0);
   int before = 0;
   for (int g0 = 0; g0 < groups; g0 += 32 * kAhead) {
     int r0[kAhead], n[kAhead];                         // kAhead warps of groups, loaded together
@@ -34,8 +34,8 @@ __device__ __forceinline__ Unit find_unit(const int32_t* __restrict__ offsets, i
       const int g = g0 + 32 * i + lane;
       r0[i] = n[i] = 0;
       if (g < groups) {
-        r0[i] = min(max(__ldg(offsets + g), 0), T);
-        const int r1 = g < G ? min(max(__ldg(offsets + g + 1), 0), T) : T;
+        r0[i] = g <= G ? min(max(__ldg(offsets + g), 0), T) : 0;
+        const int r1 = g == G ? T : min(max(__ldg(offsets + (g < G ? g + 1 : 0)), 0), T);
         n[i] = max(0, r1 - r0[i]);
       }
     }

@@ -55,7 +55,6 @@ using namespace tc;
 constexpr int kTile = 128;                             // rows per tile (MMA M)
 constexpr int kStep = 64;                              // contraction or output columns per step: 128 bytes
 constexpr int kXBytes = kTile * kStep * 2;             // 16 KB
-constexpr long long kWaitLimit = 4000000000LL;         // about 2 s at 1.9 GHz
 
 // fp32 D, BF16 A and B, M = 128; amn / bmn: the operand's M or N index is contiguous
 __device__ __forceinline__ uint32_t idesc(int n, int amn, int bmn) {
@@ -84,6 +83,7 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
+__device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void prefetch(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -159,21 +159,36 @@ struct Ring {
   }
 };
 
-// Bounded wait of one thread; after the first timeout the CTA no longer waits.
-__device__ __forceinline__ void wait_one(uint32_t bar, uint32_t parity, volatile int* failed) {
+// Waits are bounded: the first that runs out sets the CTA's flag and the device
+// error word, and the CTA no longer waits.
+struct Guard {
+  volatile int* failed;
+  long long limit;                                     // clock64 cycles
+};
+__device__ __forceinline__ void wait_one(uint32_t bar, uint32_t parity, const Guard& guard) {
   if (try_wait_at(bar, parity)) return;
   const long long t0 = clock64();
   while (!try_wait_at(bar, parity)) {
-    if (*failed) return;
-    if (clock64() - t0 > kWaitLimit) {
-      *failed = 1;
+    if (*guard.failed) return;
+    if (clock64() - t0 > guard.limit) {
+      *guard.failed = 1;
       atomicExch(&g_lora_error, 1);
       return;
     }
   }
 }
-__device__ __forceinline__ void wait_bar(uint32_t bar, uint32_t parity, volatile int* failed) {
-  wait_one(bar, parity, failed);
+__device__ __forceinline__ void wait_bar(uint32_t bar, uint32_t parity, const Guard& guard) {
+  wait_one(bar, parity, guard);
+  __syncwarp();
+}
+
+// The MMA warp's last act: every MMA that it issued has finished (bounded, even
+// after a wait has failed), so that TMEM and shared memory can go.
+__device__ __forceinline__ void finish_mmas(uint64_t* bar, uint32_t go, long long limit) {
+  commit_at(smem_u32(bar), go);
+  const long long t0 = clock64();
+  while (!try_wait_at(smem_u32(bar), 0) && clock64() - t0 < limit) {
+  }
   __syncwarp();
 }
 
@@ -214,6 +229,8 @@ struct TileArgs {
   const float* u_in;                                   // DIR 1: the forward pass's u, [T, R], or nullptr
   uint16_t* split;                                     // DIR 0: [T][s u hi, lo][R]; DIR 1: [T][v hi, lo, u hi, lo][R]
   int parts;                                           // expand: CTAs per tile
+  long long limit;                                     // of a wait, in clock64 cycles
+  int drop;                                            // error-path test: the loaders load nothing
 };
 
 __device__ __forceinline__ int rank_of(const int32_t* rank, int g, int R) {
@@ -337,7 +354,7 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
   constexpr int kStages = L::kStages, kTurn = L::kGroups, kMmaWarp = kTurn * kLoadWarps;
   constexpr uint32_t kTmemCols = RB * 64;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full[kStages], used[kStages], sums;
+  __shared__ uint64_t full[kStages], used[kStages], sums, last;
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
   __shared__ Unit unit_s;
@@ -364,6 +381,7 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
         mbar_init(&used[s], 1);
       }
       mbar_init(&sums, 1);
+      mbar_init(&last, 1);
       failed = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -382,6 +400,7 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
       asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
   };
   const Unit un = unit_s;
+  const Guard guard{&failed, a.limit};
   if (un.rows == 0) return free_tmem();                // the whole cluster leaves
   const int K1 = a.K1, R = a.R, g = un.g;
   const int lt = tid % kLoaders, group = tid / kLoaders;
@@ -407,8 +426,8 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
     Weights<RB, DIR == 0> w(a.w1, g, K1, R, rk, rp, lt, kb + group);
     Ring<kStages> at;
     for (int e = 0; e < group; ++e) at.next();
-    for (int s = group; s < nk; s += kTurn) {
-      if (s >= kStages) wait_bar(used_a + 8 * at.slot, at.parity ^ 1u, &failed);
+    for (int s = group; s < nk && !a.drop; s += kTurn) {
+      if (s >= kStages) wait_bar(used_a + 8 * at.slot, at.parity ^ 1u, guard);
       const uint32_t st = ring + at.slot * L::kStageBytes;
       rows.load(st + xo, kTurn);
       w.load(st + kXBytes, xo, kTurn);
@@ -416,6 +435,7 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
 #pragma unroll
       for (int e = 0; e < kTurn; ++e) at.next();
     }
+    cp_wait_all();
   } else {
     // ------------------------------------------------------------------ MMAs
     // Its instructions are the step's critical path: descriptors are built once
@@ -427,7 +447,7 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
     constexpr uint32_t kPer = DIR ? 2048 >> 4 : 2;     // 16 contraction indices on in the weights
 #pragma unroll 1
     for (int s = 0; s < nk; ++s) {
-      wait_bar(full_a + 8 * at.slot, at.parity, &failed);
+      wait_bar(full_a + 8 * at.slot, at.parity, guard);
       fence_async();
       const uint32_t off = at.slot * (L::kStageBytes >> 4);
 #pragma unroll
@@ -436,6 +456,7 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
       at.next();
     }
     commit_at(smem_u32(&sums), go);
+    finish_mmas(&last, go, a.limit);
   }
 
   // ---- sums: this thread's row, eight rank columns at a time ---------------------------
@@ -482,7 +503,7 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
   float4 u[2];
   if (warp < kMmaWarp) {
     load_u(first, u);
-    wait_bar(smem_u32(&sums), 0, &failed);             // every MMA has read the ring
+    wait_bar(smem_u32(&sums), 0, guard);             // every MMA has read the ring
   }
   tc_fence_after();
   if (csize == 1) {
@@ -557,7 +578,7 @@ __global__ void __launch_bounds__(Expand<RB>::kThreads, Expand<RB>::kPerSM) lora
   constexpr int kStages = L::kStages, kDrainWarps = L::kDrainWarps, kOuts = L::kOuts;
   constexpr uint32_t kTmemCols = 64 * kOuts;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full[kStages], used[kStages], operand, out_full[kOuts], out_free[kOuts];
+  __shared__ uint64_t full[kStages], used[kStages], operand, out_full[kOuts], out_free[kOuts], last;
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
   __shared__ Unit unit_s;
@@ -575,6 +596,7 @@ __global__ void __launch_bounds__(Expand<RB>::kThreads, Expand<RB>::kPerSM) lora
         mbar_init(&used[s], kDrainWarps / 2);
       }
       mbar_init(&operand, kLoaders);
+      mbar_init(&last, 1);
       for (int i = 0; i < kOuts; ++i) {
         mbar_init(&out_full[i], 1);
         mbar_init(&out_free[i], kDrainWarps / 2);
@@ -599,6 +621,7 @@ __global__ void __launch_bounds__(Expand<RB>::kThreads, Expand<RB>::kPerSM) lora
       asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
   };
   const Unit un = unit_s;
+  const Guard guard{&failed, a.limit};
   const int K2 = a.K2, R = a.R, g = un.g;
   const int c_all = (K2 + kStep - 1) / kStep, c_per = (c_all + a.parts - 1) / a.parts;
   const int cb = min(c_all, part * c_per), nc = min(c_all, cb + c_per) - cb;
@@ -651,13 +674,13 @@ __global__ void __launch_bounds__(Expand<RB>::kThreads, Expand<RB>::kPerSM) lora
     };
     // base and weights do not depend on the shrink: they go first
     const int ahead = min(nc, kStages);
-    for (int s = 0; s < ahead; ++s) step();
+    for (int s = 0; s < ahead && !a.drop; ++s) step();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int n8 = min(rp, R) / 8;                     // chunks in memory; zeros behind them up to rp / 8
 #pragma unroll
     for (int e = 0; e < RB; ++e) {
       const int c = (l & 7) + 8 * e;
-      if (c < rp / 8) {
+      if (c < rp / 8 && !a.drop) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int m = (l >> 3) + 16 * j;
@@ -668,11 +691,12 @@ __global__ void __launch_bounds__(Expand<RB>::kThreads, Expand<RB>::kPerSM) lora
         }
       }
     }
-    cp_arrive(smem_u32(&operand));
-    for (int s = ahead; s < nc; ++s) {
-      wait_bar(used_a + 8 * at.slot, at.parity ^ 1u, &failed);
+    if (!a.drop) cp_arrive(smem_u32(&operand));
+    for (int s = ahead; s < nc && !a.drop; ++s) {
+      wait_bar(used_a + 8 * at.slot, at.parity ^ 1u, guard);
       step();
     }
+    cp_wait_all();
   } else if (warp == kDrainWarps) {
     // ------------------------------------------------------------------ MMAs
     const uint32_t go = elect_one(), id = idesc(kStep, 0, DIR);
@@ -680,13 +704,13 @@ __global__ void __launch_bounds__(Expand<RB>::kThreads, Expand<RB>::kPerSM) lora
     const uint64_t du = smem_desc(op);
     const uint64_t dw0 = DIR ? desc_mn(ring + kXBytes, 8192) : smem_desc(ring + kXBytes);
     const uint32_t of = smem_u32(out_full), fr = smem_u32(out_free);
-    wait_bar(smem_u32(&operand), 0, &failed);
+    wait_bar(smem_u32(&operand), 0, guard);
 #pragma unroll 1
     for (int o = 0; o < nc; ++o) {
       const int buf = o % kOuts;
-      wait_bar(full_a + 8 * at.slot, at.parity, &failed);
+      wait_bar(full_a + 8 * at.slot, at.parity, guard);
       if (o >= kOuts) {
-        wait_bar(fr + 8 * buf, (uint32_t)(o / kOuts - 1) & 1u, &failed);
+        wait_bar(fr + 8 * buf, (uint32_t)(o / kOuts - 1) & 1u, guard);
         tc_fence_after();
       }
       fence_async();
@@ -702,6 +726,7 @@ __global__ void __launch_bounds__(Expand<RB>::kThreads, Expand<RB>::kPerSM) lora
       commit_at(of + 8 * buf, go);
       at.next();
     }
+    finish_mmas(&last, go, a.limit);
   } else {
     // ------------------------------------------------------------------ outputs
     // base (in the ring) plus product, one rounding.  The two groups of four
@@ -714,8 +739,8 @@ __global__ void __launch_bounds__(Expand<RB>::kThreads, Expand<RB>::kPerSM) lora
     for (int o = half; o < nc; o += 2) {
       const int buf = o % kOuts;
       uint8_t* xt = smem + (size_t)at.slot * L::kStageBytes;
-      wait_bar(of + 8 * buf, (uint32_t)(o / kOuts) & 1u, &failed);
-      wait_bar(full_a + 8 * at.slot, at.parity, &failed);
+      wait_bar(of + 8 * buf, (uint32_t)(o / kOuts) & 1u, guard);
+      wait_bar(full_a + 8 * at.slot, at.parity, guard);
       tc_fence_after();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -765,6 +790,8 @@ struct DwArgs {
   const int32_t *rank, *offsets, *token_of_row;
   int M[2];                                            // H, N
   int T, G, R;
+  long long limit;
+  int drop;
 };
 
 // A step is 32 rows of 256 columns: 16 KB of x or dy and RB x 8 KB of the
@@ -790,7 +817,7 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
   using D = Dw<RB>;
   constexpr int kStages = D::kStages, kRows = D::kRows;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full[kStages], used[kStages], sums;
+  __shared__ uint64_t full[kStages], used[kStages], sums, last;
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
   cg::cluster_group cl = cg::this_cluster();
@@ -838,6 +865,7 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
       mbar_init(&used[s], 1);
     }
     mbar_init(&sums, 1);
+    mbar_init(&last, 1);
     failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -851,6 +879,7 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  const Guard guard{&failed, a.limit};
 
   if (warp == kLoadWarps) {
     // ------------------------------------------------------------------ MMAs
@@ -861,7 +890,7 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
       Ring<kStages> at;
 #pragma unroll 1
       for (int s = 0; s < ns; ++s) {
-        wait_bar(full_a + 8 * at.slot, at.parity, &failed);
+        wait_bar(full_a + 8 * at.slot, at.parity, guard);
         fence_async();
         const uint32_t off = at.slot * (D::kStageBytes >> 4);
 #pragma unroll
@@ -878,6 +907,7 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
         at.next();
       }
       commit_at(smem_u32(&sums), go);
+      finish_mmas(&last, go, a.limit);
     }
     __syncwarp();
   } else {
@@ -906,13 +936,13 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
     load_tok(cur, 0);
     asm volatile("griddepcontrol.wait;" ::: "memory"); // the factors come from the shrink
     Ring<kStages> at;
-    for (int s0 = 0; s0 < ns; s0 += 4) {
+    for (int s0 = 0; s0 < ns && !a.drop; s0 += 4) {
       load_tok(nxt, s0 + 4);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int s = s0 + e;
         if (s >= ns) break;
-        if (s >= kStages) wait_bar(used_a + 8 * at.slot, at.parity ^ 1u, &failed);
+        if (s >= kStages) wait_bar(used_a + 8 * at.slot, at.parity ^ 1u, guard);
         const uint32_t st = ring + at.slot * D::kStageBytes;
         const int row = first + s * kRows;
 #pragma unroll
@@ -942,7 +972,8 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
 #pragma unroll
       for (int e = 0; e < 4; ++e) cur[e] = nxt[e];
     }
-    wait_bar(smem_u32(&sums), 0, &failed);             // every MMA has read the ring
+    cp_wait_all();
+    wait_bar(smem_u32(&sums), 0, guard);             // every MMA has read the ring
     tc_fence_after();
   }
   __syncthreads();                                     // the ring is free: partial sums take its place
@@ -1041,7 +1072,7 @@ int share(long long units, int steps, int places, int fixed, int fixed_shared, i
 
 template <int DIR, int RB>
 zmoe_status launch_tiles(TileArgs a, cudaStream_t stream) {
-  const long long units = a.T / kTile + (a.T < a.G + 1 ? a.T : a.G + 1);       // at most
+  const long long units = a.T / kTile + (a.T < a.G + 2 ? a.T : a.G + 2);       // at most
   const int tiles = (a.T + kTile - 1) / kTile + (a.T < a.G ? a.T : a.G) / 2;   // about
   using S = Shrink<RB>;
   using E = Expand<RB>;
@@ -1075,18 +1106,18 @@ zmoe_status launch_dw(const DwArgs& a, cudaStream_t stream) {
 
 zmoe_status launch_tiles(const zmoe_lora_args* p, cudaStream_t stream) {
   const TileArgs a{p->x, p->a, p->b, p->base, p->scale, p->rank, p->offsets, p->token_of_row, p->T, p->H, p->N, p->G,
-                   p->R, p->out, p->u, nullptr, reinterpret_cast<uint16_t*>(p->scratch), 1};
+                   p->R, p->out, p->u, nullptr, reinterpret_cast<uint16_t*>(p->scratch), 1, tc::wait_limit(), tc::drop_loads()};
   return p->R <= 64 ? launch_tiles<0, 1>(a, stream) : launch_tiles<0, 2>(a, stream);
 }
 
 zmoe_status launch_grad_tiles(const zmoe_lora_grad_args* p, cudaStream_t stream) {
   uint16_t* split = reinterpret_cast<uint16_t*>(p->scratch);
   const TileArgs a{p->dy, p->b, p->a, p->base, p->scale, p->rank, p->offsets, p->token_of_row, p->T, p->N, p->H, p->G,
-                   p->R, p->dx, nullptr, p->da ? p->u : nullptr, split, 1};
+                   p->R, p->dx, nullptr, p->da ? p->u : nullptr, split, 1, tc::wait_limit(), tc::drop_loads()};
   zmoe_status st = p->R <= 64 ? launch_tiles<1, 1>(a, stream) : launch_tiles<1, 2>(a, stream);
   if (st != ZMOE_OK || !p->da) return st;
   const DwArgs d{{p->x, p->dy}, split, {p->da, p->db}, p->scale, p->rank, p->offsets, p->token_of_row,
-                 {p->H, p->N}, p->T, p->G, p->R};
+                 {p->H, p->N}, p->T, p->G, p->R, tc::wait_limit(), tc::drop_loads()};
   return p->R <= 64 ? launch_dw<1>(d, stream) : launch_dw<2>(d, stream);
 }
 

@@ -5,6 +5,11 @@
 namespace zmoe {
 namespace tc {
 
+// What zmoe_debug_ffn_wait set (ffn_tc.cu): the wait limit in clock64 cycles, and
+// whether loaders issue nothing.
+long long wait_limit();
+int drop_loads();
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
