@@ -254,7 +254,7 @@ def permute(topk_idx: torch.Tensor, x: Optional[torch.Tensor], E: int, capacity:
     H = x.shape[1] if x is not None else 0
     counts, offsets = topk_idx.new_empty(E), topk_idx.new_empty(E + 1)
     row_of, tor = torch.empty_like(topk_idx), topk_idx.new_empty(max(T * k, 1))
-    xp = torch.empty(max(T * k, 1), H, dtype=torch.bfloat16, device=dev) if x is not None else None
+    xp = x.new_empty(max(T * k, 1), H, dtype=torch.bfloat16) if x is not None else None
     a = PermuteArgs(topk_idx.data_ptr(), _ptr(x), T, H, E, k, capacity, seq_len, counts.data_ptr(),
                     offsets.data_ptr(), row_of.data_ptr(), tor.data_ptr(), _ptr(xp))
     check(lib.zmoe_permute(ctypes.byref(a), _stream()), "zmoe_permute")
@@ -301,23 +301,29 @@ def combine(y: torch.Tensor, row_of: torch.Tensor, topk_w: torch.Tensor, mode: i
 _BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 
 
-def _arg(t: Optional[torch.Tensor], name: str, dtype, shape: tuple, device: int, optional: bool = False):
+def _arg(t: torch.Tensor, name: str, dtype, shape: tuple, device: int) -> int:
     """Device pointer of an argument after checking its type, shape and place."""
-    if t is None:
-        if not optional:
-            raise ValueError(f"{name}: missing")
-        return None
-    if t.dtype is not dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {shape} on cuda:{device}, "
-                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
+    if t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous():
+        return t.data_ptr()
+    raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {shape} on cuda:{device}, "
+                     f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _opt(t: Optional[torch.Tensor], name: str, dtype, shape: tuple, device: int) -> Optional[int]:
+    return None if t is None else _arg(t, name, dtype, shape, device)
 
 
 def _cuda(t: torch.Tensor, name: str, dims: int) -> int:
     """Device index of a CUDA tensor with `dims` dimensions."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != dims:
+    if not t.is_cuda or t.dim() != dims:
         raise ValueError(f"{name}: expected a CUDA tensor with {dims} dimensions")
     return t.get_device()
+
+
+def _dims(t: torch.Tensor, name: str, dims: int) -> tuple:
+    if t.dim() != dims:
+        raise ValueError(f"{name}: expected {dims} dimensions, got {t.dim()}")
+    return t.shape
 
 
 def _call(fn, args, device: int):
@@ -337,12 +343,11 @@ def permute_grad(dxp: torch.Tensor, row_of: torch.Tensor, base: Optional[torch.T
     dxp[row_of[t, j]].  base (the gradient from other paths) may be dx itself."""
     dev = _cuda(dxp, "dxp", 2)
     rows, H = dxp.shape
-    _cuda(row_of, "row_of", 2)
-    T, k = row_of.shape
+    T, k = _dims(row_of, "row_of", 2)
     if dx is None:
         dx = dxp.new_empty(T, H)
     a = PermuteGradArgs(_arg(dxp, "dxp", _BF16, (rows, H), dev), _arg(row_of, "row_of", _I32, (T, k), dev),
-                        _arg(base, "base", _BF16, (T, H), dev, True), T, H, k, rows,
+                        _opt(base, "base", _BF16, (T, H), dev), T, H, k, rows,
                         _arg(dx, "dx", _BF16, (T, H), dev))
     _call(lib.zmoe_permute_grad, a, dev)
     return dx
@@ -357,10 +362,9 @@ def combine_grad(dout: torch.Tensor, y: torch.Tensor, row_of: torch.Tensor, topk
     they were (uninitialised when dy is not given)."""
     dev = _cuda(dout, "dout", 2)
     T, H = dout.shape
-    _cuda(y, "y", 2)
-    rows = y.shape[0]
-    _cuda(row_of, "row_of", 2)
-    k = row_of.shape[1]
+    rows, k = _dims(y, "y", 2)[0], _dims(row_of, "row_of", 2)[1]
+    if x is None and mode == ROUTE_SWITCH:
+        raise ValueError("x: Switch needs it")
     if shared_gate is not None and y_shared is None:
         raise ValueError("shared_gate without y_shared")
     if dy is None:
@@ -370,10 +374,10 @@ def combine_grad(dout: torch.Tensor, y: torch.Tensor, row_of: torch.Tensor, topk
     dg = topk_w.new_empty(T) if shared_gate is not None else None
     dx = torch.empty_like(dout) if mode == ROUTE_SWITCH else None
     a = CombineGradArgs(_arg(dout, "dout", _BF16, (T, H), dev), _arg(y, "y", _BF16, (rows, H), dev),
-                        _arg(y_shared, "y_shared", _BF16, (T, H), dev, True),
-                        _arg(shared_gate, "shared_gate", _F32, (T,), dev, True),
+                        _opt(y_shared, "y_shared", _BF16, (T, H), dev),
+                        _opt(shared_gate, "shared_gate", _F32, (T,), dev),
                         _arg(row_of, "row_of", _I32, (T, k), dev), _arg(topk_w, "topk_w", _F32, (T, k), dev),
-                        _arg(x, "x", _BF16, (T, H), dev, mode != ROUTE_SWITCH), T, H, k, mode, rows,
+                        _opt(x, "x", _BF16, (T, H), dev), T, H, k, mode, rows,
                         _arg(dy, "dy", _BF16, (rows, H), dev), dw.data_ptr(), _ptr(dysh), _ptr(dg), _ptr(dx))
     _call(lib.zmoe_combine_grad, a, dev)
     return dy, dw, dysh, dg, dx
@@ -393,13 +397,11 @@ def lora_plan(adapter: torch.Tensor, G: int):
 
 
 def _adapters(a: torch.Tensor, b: torch.Tensor, scale, rank, offsets, token_of_row, T: int, dev):
-    _cuda(a, "a", 3)
-    _cuda(b, "b", 3)
-    G, R, H = a.shape
-    N = b.shape[1]
+    G, R, H = _dims(a, "a", 3)
+    N = _dims(b, "b", 3)[1]
     return (G, R, H, N, _arg(a, "a", _BF16, (G, R, H), dev), _arg(b, "b", _BF16, (G, N, R), dev),
-            _arg(scale, "scale", _F32, (G,), dev, True), _arg(rank, "rank", _I32, (G,), dev, True),
-            _arg(offsets, "offsets", _I32, (G + 1,), dev), _arg(token_of_row, "token_of_row", _I32, (T,), dev, True))
+            _opt(scale, "scale", _F32, (G,), dev), _opt(rank, "rank", _I32, (G,), dev),
+            _arg(offsets, "offsets", _I32, (G + 1,), dev), _opt(token_of_row, "token_of_row", _I32, (T,), dev))
 
 
 def lora(x: torch.Tensor, base: Optional[torch.Tensor], a: torch.Tensor, b: torch.Tensor,
@@ -418,8 +420,8 @@ def lora(x: torch.Tensor, base: Optional[torch.Tensor], a: torch.Tensor, b: torc
     if out is None:
         out = x.new_empty(T, N)
     scratch = x.new_empty(T, 2 * R) if T > _lib.LORA_ROWS else None
-    args = LoraArgs(_arg(x, "x", _BF16, (T, H), dev), _arg(base, "base", _BF16, (T, N), dev, True), pa, pb, ps, pr,
-                    po, pt, T, H, N, G, R, _arg(out, "out", _BF16, (T, N), dev), _arg(u, "u", _F32, (T, R), dev, True),
+    args = LoraArgs(_arg(x, "x", _BF16, (T, H), dev), _opt(base, "base", _BF16, (T, N), dev), pa, pb, ps, pr,
+                    po, pt, T, H, N, G, R, _arg(out, "out", _BF16, (T, N), dev), _opt(u, "u", _F32, (T, R), dev),
                     _ptr(scratch))
     _call(lib.zmoe_lora, args, dev)
     return out
@@ -441,7 +443,7 @@ def lora_grad(dy: torch.Tensor, x: torch.Tensor, u: torch.Tensor, a: torch.Tenso
     scratch = dy.new_empty(T, 4 * R)
     args = LoraGradArgs(_arg(dy, "dy", _BF16, (T, N), dev), _arg(x, "x", _BF16, (T, H), dev),
                         _arg(u, "u", _F32, (T, R), dev), pa, pb, ps, pr, po, pt,
-                        _arg(base, "base", _BF16, (T, H), dev, True), T, H, N, G, R,
+                        _opt(base, "base", _BF16, (T, H), dev), T, H, N, G, R,
                         _arg(dx, "dx", _BF16, (T, H), dev), da.data_ptr(), db.data_ptr(), scratch.data_ptr())
     _call(lib.zmoe_lora_grad, args, dev)
     return dx, da, db
