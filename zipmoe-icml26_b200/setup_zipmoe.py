@@ -1,5 +1,5 @@
-"""Builds the `ZipMoE` Python module (csrc/zipmoe_module.cpp) in place, linked
-against libzmoe.so in this directory:
+"""Builds the `ZipMoE` Python module (csrc/zipmoe_module.cpp) and `zmoe._ops`
+(csrc/ops_module.cpp) in place, linked against libzmoe.so in this directory:
 
     python setup_zipmoe.py build_ext --inplace --build-temp _build/pyext
 """
@@ -11,16 +11,23 @@ from torch.utils.cpp_extension import BuildExtension, CUDAExtension
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 
-setup(
-    name="ZipMoE",
-    ext_modules=[CUDAExtension(
-        "ZipMoE",
-        [os.path.join("csrc", "zipmoe_module.cpp")],
+
+def extension(name, source, rpath):
+    return CUDAExtension(
+        name,
+        [os.path.join("csrc", source)],
         include_dirs=[os.path.join(ROOT, "include")],
         library_dirs=[HERE],
         libraries=["zmoe"],
         extra_compile_args={"cxx": ["-O2", "-g0", "-Wall", "-Wno-unused-parameter"]},
-        extra_link_args=["-Wl,-rpath,$ORIGIN"],
-    )],
+        extra_link_args=["-Wl,-rpath," + rpath],
+    )
+
+
+setup(
+    name="ZipMoE",
+    packages=[],
+    ext_modules=[extension("ZipMoE", "zipmoe_module.cpp", "$ORIGIN"),
+                 extension("zmoe._ops", "ops_module.cpp", "$ORIGIN/..")],
     cmdclass={"build_ext": BuildExtension},
 )

@@ -12,8 +12,8 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import (CombineArgs, CombineGradArgs, FfnArgs, LoraArgs, LoraGradArgs, PermuteArgs, PermuteGradArgs,
-                   RouterArgs, ZmoeChunk, ZmoeEncChunk, check, lib)
+from . import _ops  # C++ side of the calls whose host time counts (csrc/ops_module.cpp)
+from ._lib import CombineArgs, FfnArgs, RouterArgs, ZmoeChunk, ZmoeEncChunk, check, lib
 
 ROUTE_QWEN, ROUTE_DEEPSEEK, ROUTE_SWITCH = 0, 1, 2
 
@@ -248,17 +248,7 @@ def router(x: torch.Tensor, w: torch.Tensor, k: int, mode: int, bias: Optional[t
 def permute(topk_idx: torch.Tensor, x: Optional[torch.Tensor], E: int, capacity: int = 0, seq_len: int = 0):
     """Returns counts, offsets, row_of, token_of_row, xp.  topk_idx is updated
     in place (-1 for capacity drops)."""
-    _need(topk_idx, torch.int32, "topk_idx")
-    T, k = topk_idx.shape
-    dev = topk_idx.device
-    H = x.shape[1] if x is not None else 0
-    counts, offsets = topk_idx.new_empty(E), topk_idx.new_empty(E + 1)
-    row_of, tor = torch.empty_like(topk_idx), topk_idx.new_empty(max(T * k, 1))
-    xp = x.new_empty(max(T * k, 1), H, dtype=torch.bfloat16) if x is not None else None
-    a = PermuteArgs(topk_idx.data_ptr(), _ptr(x), T, H, E, k, capacity, seq_len, counts.data_ptr(),
-                    offsets.data_ptr(), row_of.data_ptr(), tor.data_ptr(), _ptr(xp))
-    check(lib.zmoe_permute(ctypes.byref(a), _stream()), "zmoe_permute")
-    return counts, offsets, row_of, tor, xp
+    return _ops.permute(topk_idx, x, E, capacity, seq_len)
 
 
 def weight_table(mats: Sequence[Sequence[Optional[torch.Tensor]]], device=None) -> torch.Tensor:
@@ -298,59 +288,11 @@ def combine(y: torch.Tensor, row_of: torch.Tensor, topk_w: torch.Tensor, mode: i
 # ---------------------------------------------------------------------------
 # gradients of permute and combine, low-rank adapters
 # ---------------------------------------------------------------------------
-_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
-
-
-def _arg(t: torch.Tensor, name: str, dtype, shape: tuple, device: int) -> int:
-    """Device pointer of an argument after checking its type, shape and place."""
-    if t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous():
-        return t.data_ptr()
-    raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {shape} on cuda:{device}, "
-                     f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-
-
-def _opt(t: Optional[torch.Tensor], name: str, dtype, shape: tuple, device: int) -> Optional[int]:
-    return None if t is None else _arg(t, name, dtype, shape, device)
-
-
-def _cuda(t: torch.Tensor, name: str, dims: int) -> int:
-    """Device index of a CUDA tensor with `dims` dimensions."""
-    if not t.is_cuda or t.dim() != dims:
-        raise ValueError(f"{name}: expected a CUDA tensor with {dims} dimensions")
-    return t.get_device()
-
-
-def _dims(t: torch.Tensor, name: str, dims: int) -> tuple:
-    if t.dim() != dims:
-        raise ValueError(f"{name}: expected {dims} dimensions, got {t.dim()}")
-    return t.shape
-
-
-def _call(fn, args, device: int):
-    """Runs an entry point on the arguments' device and that device's current stream."""
-    if device == torch._C._cuda_getDevice():
-        status = fn(ctypes.byref(args), _stream())
-    else:
-        with torch.cuda.device(device):
-            status = fn(ctypes.byref(args), _stream())
-    if status:
-        check(status, fn.__name__)
-
-
 def permute_grad(dxp: torch.Tensor, row_of: torch.Tensor, base: Optional[torch.Tensor] = None,
                  dx: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Gradient of permute's gather (zmoe_permute_grad): dx[t] = base[t] + sum_j
     dxp[row_of[t, j]].  base (the gradient from other paths) may be dx itself."""
-    dev = _cuda(dxp, "dxp", 2)
-    rows, H = dxp.shape
-    T, k = _dims(row_of, "row_of", 2)
-    if dx is None:
-        dx = dxp.new_empty(T, H)
-    a = PermuteGradArgs(_arg(dxp, "dxp", _BF16, (rows, H), dev), _arg(row_of, "row_of", _I32, (T, k), dev),
-                        _opt(base, "base", _BF16, (T, H), dev), T, H, k, rows,
-                        _arg(dx, "dx", _BF16, (T, H), dev))
-    _call(lib.zmoe_permute_grad, a, dev)
-    return dx
+    return _ops.permute_grad(dxp, row_of, base, dx)
 
 
 def combine_grad(dout: torch.Tensor, y: torch.Tensor, row_of: torch.Tensor, topk_w: torch.Tensor, mode: int,
@@ -360,48 +302,14 @@ def combine_grad(dout: torch.Tensor, y: torch.Tensor, row_of: torch.Tensor, topk
     dshared_gate, dx; the last three are None without y_shared, without
     shared_gate and outside Switch.  Rows of dy that no slot names are left as
     they were (uninitialised when dy is not given)."""
-    dev = _cuda(dout, "dout", 2)
-    T, H = dout.shape
-    rows, k = _dims(y, "y", 2)[0], _dims(row_of, "row_of", 2)[1]
-    if x is None and mode == ROUTE_SWITCH:
-        raise ValueError("x: Switch needs it")
-    if shared_gate is not None and y_shared is None:
-        raise ValueError("shared_gate without y_shared")
-    if dy is None:
-        dy = torch.empty_like(y)
-    dw = topk_w.new_empty(T, k)
-    dysh = torch.empty_like(dout) if y_shared is not None else None
-    dg = topk_w.new_empty(T) if shared_gate is not None else None
-    dx = torch.empty_like(dout) if mode == ROUTE_SWITCH else None
-    a = CombineGradArgs(_arg(dout, "dout", _BF16, (T, H), dev), _arg(y, "y", _BF16, (rows, H), dev),
-                        _opt(y_shared, "y_shared", _BF16, (T, H), dev),
-                        _opt(shared_gate, "shared_gate", _F32, (T,), dev),
-                        _arg(row_of, "row_of", _I32, (T, k), dev), _arg(topk_w, "topk_w", _F32, (T, k), dev),
-                        _opt(x, "x", _BF16, (T, H), dev), T, H, k, mode, rows,
-                        _arg(dy, "dy", _BF16, (rows, H), dev), dw.data_ptr(), _ptr(dysh), _ptr(dg), _ptr(dx))
-    _call(lib.zmoe_combine_grad, a, dev)
-    return dy, dw, dysh, dg, dx
+    return _ops.combine_grad(dout, y, row_of, topk_w, mode, y_shared, shared_gate, x, dy)
 
 
 def lora_plan(adapter: torch.Tensor, G: int):
     """Rows of a batch grouped by adapter (zmoe_lora_plan): adapter[t] in [0, G),
     anything else for a token without one.  Returns offsets [G + 1] and
     token_of_row [T], which serve every projection of the step."""
-    dev = _cuda(adapter, "adapter", 1)
-    T = adapter.shape[0]
-    offsets, tor = adapter.new_empty(max(G, 0) + 1), adapter.new_empty(T)
-    ids = _arg(adapter, "adapter", _I32, (T,), dev)
-    with torch.cuda.device(dev):
-        check(lib.zmoe_lora_plan(ids, T, G, offsets.data_ptr(), tor.data_ptr(), _stream()), "zmoe_lora_plan")
-    return offsets, tor
-
-
-def _adapters(a: torch.Tensor, b: torch.Tensor, scale, rank, offsets, token_of_row, T: int, dev):
-    G, R, H = _dims(a, "a", 3)
-    N = _dims(b, "b", 3)[1]
-    return (G, R, H, N, _arg(a, "a", _BF16, (G, R, H), dev), _arg(b, "b", _BF16, (G, N, R), dev),
-            _opt(scale, "scale", _F32, (G,), dev), _opt(rank, "rank", _I32, (G,), dev),
-            _arg(offsets, "offsets", _I32, (G + 1,), dev), _opt(token_of_row, "token_of_row", _I32, (T,), dev))
+    return _ops.lora_plan(adapter, G)
 
 
 def lora(x: torch.Tensor, base: Optional[torch.Tensor], a: torch.Tensor, b: torch.Tensor,
@@ -414,17 +322,7 @@ def lora(x: torch.Tensor, base: Optional[torch.Tensor], a: torch.Tensor, b: torc
     offsets and token_of_row come from lora_plan, or offsets from permute when
     x holds its gathered rows (an adapter per expert).  out may be base; base
     None counts as zeros.  u (fp32 [T, R]) receives x a^T for lora_grad."""
-    dev = _cuda(x, "x", 2)
-    T = x.shape[0]
-    G, R, H, N, pa, pb, ps, pr, po, pt = _adapters(a, b, scale, rank, offsets, token_of_row, T, dev)
-    if out is None:
-        out = x.new_empty(T, N)
-    scratch = x.new_empty(T, 2 * R) if T > _lib.LORA_ROWS else None
-    args = LoraArgs(_arg(x, "x", _BF16, (T, H), dev), _opt(base, "base", _BF16, (T, N), dev), pa, pb, ps, pr,
-                    po, pt, T, H, N, G, R, _arg(out, "out", _BF16, (T, N), dev), _opt(u, "u", _F32, (T, R), dev),
-                    _ptr(scratch))
-    _call(lib.zmoe_lora, args, dev)
-    return out
+    return _ops.lora(x, base, a, b, scale, offsets, token_of_row, rank, out, u)
 
 
 def lora_grad(dy: torch.Tensor, x: torch.Tensor, u: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
@@ -434,16 +332,4 @@ def lora_grad(dy: torch.Tensor, x: torch.Tensor, u: torch.Tensor, a: torch.Tenso
     """Gradient of lora (zmoe_lora_grad) from its u: returns dx = base + v a, da and
     db.  base (the gradient through the shared projection) may be dx itself;
     the gradient of lora's own base is dy."""
-    dev = _cuda(dy, "dy", 2)
-    T = dy.shape[0]
-    G, R, H, N, pa, pb, ps, pr, po, pt = _adapters(a, b, scale, rank, offsets, token_of_row, T, dev)
-    if dx is None:
-        dx = dy.new_empty(T, H)
-    da, db = torch.empty_like(a), torch.empty_like(b)
-    scratch = dy.new_empty(T, 4 * R)
-    args = LoraGradArgs(_arg(dy, "dy", _BF16, (T, N), dev), _arg(x, "x", _BF16, (T, H), dev),
-                        _arg(u, "u", _F32, (T, R), dev), pa, pb, ps, pr, po, pt,
-                        _opt(base, "base", _BF16, (T, H), dev), T, H, N, G, R,
-                        _arg(dx, "dx", _BF16, (T, H), dev), da.data_ptr(), db.data_ptr(), scratch.data_ptr())
-    _call(lib.zmoe_lora_grad, args, dev)
-    return dx, da, db
+    return _ops.lora_grad(dy, x, u, a, b, scale, offsets, token_of_row, rank, base, dx)
