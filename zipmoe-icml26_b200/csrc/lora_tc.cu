@@ -14,7 +14,7 @@
 //                       the contraction, one tile of 256 columns of x or dy per
 //                       cluster, whose CTAs share the rows.
 // (A single kernel for shrink and expand, with u kept in TMEM, measured slower:
-// 31.5 against 29 us for 8191 rows of 2048 in and out at rank 64, 40 against 20 us
+// 31.5 against 29 us for 8191 rows of 2048 in and out at rank 64, 25 against 17 us
 // for 2047 rows of 2048 in and 5632 out at rank 16: tiles of whole rows leave SMs
 // without work.)
 //
@@ -806,8 +806,9 @@ struct DwArgs {
 
 // A step is 32 rows of 256 columns: 16 KB of x or dy and RB x 8 KB of the
 // factor's two halves.  (With 128 columns the factor is read twice as often and
-// there are twice as many CTAs to set up: 40 against 30 us for 60 groups of
-// 273 rows, 2048 and 1408 columns, rank 32.)
+// there are twice as many CTAs to set up: 39 against 36 us for 60 groups of
+// 273 rows, 2048 and 1408 columns, rank 32; 13.3 against 14.9 us for one group
+// of 2047 rows.)
 template <int RB>
 struct Dw {
   static constexpr int kRows = 32, kCols = 2 * kTile;

@@ -10,7 +10,7 @@
 // Without a capacity the order is a stable counting sort of the (token, slot)
 // pairs by expert.  Each warp of a cluster of CTAs takes a run of tokens, and
 // counts its experts in its own shared-memory row (lanes with the same expert
-// find each other with match.any, so a step of 32 pairs is one add per expert
+// find each other by votes, so a step of 32 pairs is one add per expert
 // present); prefixes over warps, CTAs (through distributed shared memory) and
 // experts turn the counts into first rows, and a second walk over the same
 // pairs hands the rows out in order.  No atomics: the result does not depend
@@ -142,6 +142,9 @@ constexpr int kSortE = 1024;          // experts: one per thread in the scan, 12
 constexpr int kSortCluster = 16;      // the steps are bound by instruction issue: 98 thousand
                                       // pairs took 19 us on 8 SMs, 12 on 16
 constexpr int kFusedPairs = 2048;     // pairs every CTA of the fused launch sorts for itself
+                                      // (64 experts, rows of 2048, us, fused against two launches: 64 pairs of 4 a
+                                      // token 5.6 and 6.4, of 8 a token 6.7 and 6.4; 2048 pairs 7.7 and 9.0, 8.7 and
+                                      // 8.7; 4096 pairs 12.9 and 12.8, 12.9 and 12.3; 8192 pairs 21.5 and 19.6)
 constexpr int kHold = 16;             // steps of a warp whose pairs stay in registers between the two walks
 constexpr unsigned kFull = 0xffffffffu;
 
@@ -190,7 +193,7 @@ __device__ void sort_pairs(const SortArgs& a, int rank, int csize, int* smem, bo
   };
   auto pack = [&](int e) -> int {
     // lanes with the same expert: one vote per bit of it (a match.any instead
-    // took 0.4 us more per step of an SM's warps)
+    // took 0.3 us less for 256 pairs and 2 us more for 8192 on one SM)
     unsigned m = __ballot_sync(kFull, e >= 0);
 #pragma unroll
     for (int b = 0; b < 10; ++b) {
@@ -319,6 +322,7 @@ __global__ void __launch_bounds__(kSortThreads)
 sort_kernel(const SortArgs a) {
   extern __shared__ int sort_smem_raw[];
   cg::cluster_group cl = cg::this_cluster();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the copy may load x meanwhile
   sort_pairs(a, (int)cl.block_rank(), (int)cl.num_blocks(), sort_smem_raw, true, nullptr);
   // the last remote reads happened before the base scan's barriers of each
   // CTA; wait for the cluster so that no CTA leaves while its totals are read
@@ -431,7 +435,7 @@ zmoe_status launch_permute(const zmoe_permute_args* a, cudaStream_t stream) {
   bool copies_tokens = false;
   if (a->capacity <= 0 && a->E <= kSortE && a->k <= 32) {
     SortArgs sa{a->topk_idx, a->T, a->k, a->E, 0, a->counts, a->offsets, a->row_of, a->token_of_row};
-    if (a->xp && a->T * a->k <= kFusedPairs && vec > 0) {
+    if (a->xp && a->T * a->k <= kFusedPairs && vec > 0 && (long long)a->T * vec < 1 << 30) {
       st = allow_smem<sort_gather_kernel>();
       if (st != ZMOE_OK) return st;
       const size_t smem = sort_smem(a->E) + sizeof(int32_t) * (size_t)a->T * a->k;
