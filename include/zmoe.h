@@ -295,13 +295,14 @@ zmoe_status zmoe_combine_grad(const zmoe_combine_grad_args* a, zmoe_stream_t str
  * with base = the shared projection's output.  Rows are grouped by adapter:
  * rows offsets[g] .. offsets[g + 1] belong to adapter g, row r is token
  * token_of_row[r] (NULL: row r is token r, as for zmoe_permute's gathered
- * rows with an adapter per expert).  Rows outside [offsets[0], offsets[G]) use no
+ * rows with an adapter per expert), every token in one row.  Rows outside [offsets[0], offsets[G]) use no
  * adapter: out = base.  rank[g] <= R is the rank of adapter g: rows of A_g and columns
  * of B_g from rank[g] on are not used, whatever they hold.
  * ------------------------------------------------------------------------ */
 /* Rows of a batch from each token's adapter id: offsets [G + 1] and
  * token_of_row [T], tokens ascending inside an adapter; ids outside [0, G) use
- * no adapter and come last.  The plan serves every projection of a step. */
+ * no adapter and come last.  The plan serves every projection of a step.
+ * G <= 1023. */
 zmoe_status zmoe_lora_plan(const int32_t* adapter, int T, int G, int32_t* offsets, int32_t* token_of_row,
                            zmoe_stream_t stream);
 
@@ -317,7 +318,7 @@ typedef struct zmoe_lora_args {
   const int32_t* rank;        /* [G] or NULL (R); values are clamped to [0, R] */
   const int32_t* offsets;     /* [G + 1] device */
   const int32_t* token_of_row;/* [T] device or NULL */
-  int T, H, N, G, R;          /* H, N, R multiples of 8; R <= ZMOE_LORA_MAX_RANK */
+  int T, H, N, G, R;          /* H, N, R multiples of 8; H, N <= 32768; R <= ZMOE_LORA_MAX_RANK; T <= 2^30 */
   uint16_t* out;              /* [T, N] BF16 */
   float* u;                   /* [T, R] fp32 out by row, or NULL: x A^T, kept for zmoe_lora_grad; columns from
                                  the rank on are 0, rows behind the last adapter's are left as they were */
@@ -330,7 +331,8 @@ zmoe_status zmoe_lora(const zmoe_lora_args* a, zmoe_stream_t stream);
  *   dx[t] = base[t] + v A      dA_g = sum of v^T x over the rows of g      dB_g = scale * sum of dy^T u
  * (the gradient of zmoe_lora's base is dy itself).  Tokens without adapter:
  * dx = base.  da and db are written whole: zeros for adapters without rows and
- * from the rank on.  dx, or da and db, may be NULL. */
+ * from the rank on.  dx, or da and db, may be NULL; dx is neither dy nor x.
+ * Sizes as for zmoe_lora, and G <= 65535. */
 typedef struct zmoe_lora_grad_args {
   const uint16_t* dy;         /* [T, N] BF16 */
   const uint16_t* x;          /* [T, H] BF16 */

@@ -239,3 +239,27 @@ def test_wait_timeout_is_reported_and_context_survives(R):
     torch.cuda.synchronize()
     assert error() == 0
     assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_token_lists_of_many_rows():
+    # 242 thousand tiles, small whole numbers: every sum and output is exact (at most 256)
+    ops = _ops()
+    T, D, G = 31_000_000, 8, 2
+    offsets = torch.tensor([0, 13, T - 5], dtype=torch.int32, device="cuda")
+    tor = torch.arange(T - 1, -1, -1, dtype=torch.int32, device="cuda")
+    x = (torch.arange(T * D, device="cuda", dtype=torch.int32) % 5).to(BF).view(T, D)
+    g = torch.Generator().manual_seed(3)
+    a = torch.randint(-1, 2, (G, D, D), generator=g).to(BF).cuda()
+    b = torch.eye(D, dtype=BF).flip(0).repeat(G, 1, 1).contiguous().cuda()
+    u = torch.zeros(T, D, device="cuda")
+    out = ops.lora(x, x, a, b, None, offsets, tor, u=u)
+    dx, da, db = ops.lora_grad(x, x, u, a, b, None, offsets, tor)
+    for g0, r0, r1 in ((0, 0, 13), (1, 13, T - 5)):
+        xr = x[T - r1:T - r0].float()                  # tokens T - 1 - r
+        w, bw = a[g0].float(), b[g0].float()
+        assert torch.equal(out[T - r1:T - r0].float(), xr + xr @ w.T @ bw.T)
+        assert torch.equal(dx[T - r1:T - r0].float(), xr @ bw @ w)
+        assert torch.equal(u[r0:r1], (xr @ w.T).flip(0))
+    assert torch.equal(out[:5], x[:5]) and not dx[:5].any() and not u[T - 5:].any()
+    xr = x[T - 13:].float()
+    assert torch.equal(da[0], ((xr @ b[0].float()).T @ xr).to(BF)) and torch.equal(db[0], (xr.T @ (xr @ a[0].float().T)).to(BF))

@@ -93,3 +93,17 @@ def test_statements_agree_with_autograd():
     got = adapters.lora_grad(dy, x, torch.nan_to_num(u), a, b, s, offsets, tor, rank)
     for n, t in (("dx", xs), ("da", am), ("db", bm)):
         assert torch.allclose(got[n][0], t.grad), n
+
+
+def test_refuses_lengths_and_aliases():
+    L = _lib()
+    ok = dict(x=P, base=P, a=P, b=P, scale=P, rank=None, offsets=P, token_of_row=None, T=4, H=16, N=16, G=2, R=8, out=P, scratch=P)
+    _refused(L.lib.zmoe_lora, L.LoraArgs(**dict(ok, T=2 ** 30 + 1)), b"above")
+    Q = 2 * P
+    ok = dict(dy=P, x=P, u=P, a=P, b=P, scale=P, rank=None, offsets=P, token_of_row=None, base=None, T=4, H=16, N=16,
+              G=2, R=8, dx=Q, da=Q, db=Q, scratch=Q)
+    for kw, text in (({"T": 2 ** 30 + 1}, b"above"), ({"dy": Q}, b"must not be"), ({"x": Q}, b"must not be")):
+        _refused(L.lib.zmoe_lora_grad, L.LoraGradArgs(**dict(ok, **kw)), text)
+    assert L.lib.zmoe_lora_plan(P, 2 ** 31 - 1, 3, P, P, None) == 1
+    _refused(L.lib.zmoe_permute, L.PermuteArgs(topk_idx=P, x=None, T=2 ** 31 - 1, H=0, k=1, E=4, capacity=0, seq_len=0,
+                                               counts=P, offsets=P, row_of=P, token_of_row=P, xp=None), b"too many")

@@ -244,6 +244,7 @@ zmoe_status launch_lora(const zmoe_lora_args* a, cudaStream_t stream) {
   ZMOE_CHECK_ARG(aligned16(a->x) && aligned16(a->base) && aligned16(a->a) && aligned16(a->b) && aligned16(a->out) &&
                      aligned16(a->u) && aligned16(a->scratch), "lora: rows must be 16-byte aligned");
   ZMOE_CHECK_ARG(a->H <= kMaxCols && a->N <= kMaxCols, "lora: H=%d or N=%d above %d", a->H, a->N, kMaxCols);
+  ZMOE_CHECK_ARG(a->T <= kMaxT, "lora: T=%d above %d", a->T, kMaxT);
   // Few rows for each adapter: the rows kernel; else tiles of 128.  Measured (us, rows
   // against tiles, 2048 in and out): 512 rows 11.1 and 11.2 with one adapter of rank
   // 64, 12.5 and 24.7 with 128 of rank 16; 1024 rows 17.2 and 13.9, 11.7 and 12.9 at
@@ -279,6 +280,7 @@ zmoe_status launch_lora_grad(const zmoe_lora_grad_args* a, cudaStream_t stream) 
   ZMOE_CHECK_ARG((a->da == nullptr) == (a->db == nullptr), "lora_grad: da and db go together");
   ZMOE_CHECK_ARG(a->dx || a->da, "lora_grad: no output");
   ZMOE_CHECK_ARG(a->G <= 65535, "lora_grad: G=%d above 65535", a->G);
+  ZMOE_CHECK_ARG(a->T <= kMaxT, "lora_grad: T=%d above %d", a->T, kMaxT);
   if (a->T == 0) {
     if (a->da) {
       ZMOE_CUDA_RET(cudaMemsetAsync(a->da, 0, sizeof(uint16_t) * (size_t)a->G * a->R * a->H, stream));
@@ -290,6 +292,8 @@ zmoe_status launch_lora_grad(const zmoe_lora_grad_args* a, cudaStream_t stream) 
   ZMOE_CHECK_ARG(aligned16(a->dy) && aligned16(a->x) && aligned16(a->u) && aligned16(a->a) && aligned16(a->b) &&
                      aligned16(a->base) && aligned16(a->dx) && aligned16(a->da) && aligned16(a->db) && aligned16(a->scratch),
                  "lora_grad: rows must be 16-byte aligned");
+  // dA and dB read dy and x after dx is written
+  ZMOE_CHECK_ARG(!a->dx || !a->da || (a->dx != a->dy && a->dx != a->x), "lora_grad: dx must not be dy or x");
   return launch_grad_tiles(a, stream);
 }
 

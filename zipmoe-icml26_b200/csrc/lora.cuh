@@ -7,6 +7,7 @@ namespace lora {
 
 constexpr int kThreads = 256;
 constexpr int kMaxCols = 32768;                        // H and N
+constexpr int kMaxT = 1 << 30;                         // row and tile indexes are int
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kAhead = 4;                              // of find_unit
 

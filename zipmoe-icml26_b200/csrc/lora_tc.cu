@@ -365,7 +365,8 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
   // the token list, a share a CTA, and the ranks and scales come to L2 while the
   // unit is looked for, instead of one after the other behind it
   if (a.token_of_row)
-    for (int i = 32 * (blockIdx.x * L::kThreads + tid); i < a.T; i += 32 * gridDim.x * L::kThreads) prefetch(a.token_of_row + i);
+    for (long long i = 32LL * (blockIdx.x * (long long)L::kThreads + tid); i < a.T; i += 32LL * gridDim.x * L::kThreads)
+      prefetch(a.token_of_row + i);
   if (32 * tid < a.G) {
     if (a.rank) prefetch(a.rank + 32 * tid);
     if (a.scale) prefetch(a.scale + 32 * tid);

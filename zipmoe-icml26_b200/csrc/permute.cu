@@ -39,6 +39,7 @@ namespace zmoe {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kMaxT = 0x7fffffff - kThreads;           // a step behind the last token still is an int
 
 // Exclusive block scan of v (0/1 flags); returns the prefix, *total gets the sum.
 __device__ __forceinline__ int block_exclusive_scan(int v, int* warp_sums, int* total) {
@@ -185,8 +186,9 @@ __device__ void sort_pairs(const SortArgs& a, int rank, int csize, int* smem, bo
   // A step's pair of this lane as seen by the warp: expert, earlier lanes with
   // the same expert << 10, lanes with it << 16; -1: no row, -2: no pair.
   auto load = [&](int s) -> int {
+    if (!used || s >= s1) return -2;
     const int t = s * tp + tl;
-    if (!used || s >= s1 || t >= a.T) return -2;
+    if (t >= a.T) return -2;
     const int e = __ldg(a.idx + (size_t)t * k + jl);
     if (a.rest) return (unsigned)e < (unsigned)(E - 1) ? e : E - 1;
     return (unsigned)e < (unsigned)E ? e : -1;
@@ -288,11 +290,11 @@ __device__ void sort_pairs(const SortArgs& a, int rank, int csize, int* smem, bo
   __syncthreads();
 
   auto place = [&](int s, int v) {
-    const int t = s * tp + tl;
     const int row = v >= 0 ? base[v & 1023] + my[v & 1023] + (v >> 10 & 63) : -1;
     __syncwarp();
     count(v);
     if (v >= -1) {
+      const int t = s * tp + tl;
       if (rows_s) rows_s[t * k + jl] = row;
       if (write) {
         if (a.row_of) a.row_of[(size_t)t * k + jl] = row;
@@ -363,12 +365,19 @@ scatter_rows_kernel(const uint4* __restrict__ x, int T, int vec, int k, const in
   if (t < (size_t)T) v = __ldcs(x + t * vec + c);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (t >= (size_t)T) return;
-  for (int j = 0; j < k; ++j) {
-    const int r = row_of[t * k + j];
-    if ((unsigned)r < (unsigned)max_rows) {
-      __stcs(xp + (size_t)r * vec + c, v);
-      if (c == 0 && token_of_row) token_of_row[r] = (int)t;
+  for (int j0 = 0; j0 < k; j0 += 4) {
+    int r[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {                      // asm: not before the wait, not from a read-only cache
+      r[j] = -1;
+      if (j0 + j < k) asm volatile("ld.global.b32 %0, [%1];" : "=r"(r[j]) : "l"(row_of + t * k + j0 + j) : "memory");
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if ((unsigned)r[j] < (unsigned)max_rows) {
+        __stcs(xp + (size_t)r[j] * vec + c, v);
+        if (c == 0 && token_of_row) token_of_row[r[j]] = (int)t;
+      }
   }
 }
 
@@ -429,7 +438,7 @@ zmoe_status launch_permute(const zmoe_permute_args* a, cudaStream_t stream) {
     ZMOE_CUDA_RET(cudaMemsetAsync(a->offsets, 0, sizeof(int32_t) * (a->E + 1), stream));
     return ZMOE_OK;
   }
-  ZMOE_CHECK_ARG((long long)a->T * a->k < (1LL << 31), "permute: T=%d x k=%d pairs are too many", a->T, a->k);
+  ZMOE_CHECK_ARG(a->T <= kMaxT && (long long)a->T * a->k < (1LL << 31), "permute: T=%d x k=%d pairs are too many", a->T, a->k);
   const int vec = a->H / 8;
   zmoe_status st;
   bool copies_tokens = false;
@@ -479,6 +488,7 @@ zmoe_status launch_lora_plan(const int32_t* adapter, int T, int G, int32_t* offs
                              cudaStream_t stream) {
   ZMOE_CHECK_ARG(G >= 1 && G < kSortE, "lora_plan: G=%d outside [1, %d]", G, kSortE - 1);
   ZMOE_CHECK_ARG(T >= 0 && offsets && (T == 0 || (adapter && token_of_row)), "lora_plan: null pointer or negative T");
+  ZMOE_CHECK_ARG(T <= kMaxT, "lora_plan: T=%d above %d", T, kMaxT);
   if (T == 0) {
     ZMOE_CUDA_RET(cudaMemsetAsync(offsets, 0, sizeof(int32_t) * (size_t)(G + 1), stream));
     return ZMOE_OK;
