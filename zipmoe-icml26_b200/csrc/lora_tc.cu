@@ -583,7 +583,6 @@ __global__ void __launch_bounds__(Expand<RB>::kThreads, Expand<RB>::kPerSM) lora
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
   __shared__ Unit unit_s;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int index = (int)(gridDim.x - 1 - blockIdx.x), part = index % a.parts;
   if (warp == 0) {
@@ -687,6 +686,10 @@ __global__ void __launch_bounds__(Expand<RB>::kThreads, Expand<RB>::kPerSM) lora
     const int ahead = min(nc, kStages);
     for (int s = 0; s < ahead && !a.drop; ++s) step();
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (DIR == 1 && l == 0) {                          // the shrink has ended: dA and dB may begin
+      __threadfence();
+      asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    }
     const int n8 = min(rp, R) / 8;                     // chunks in memory; zeros behind them up to rp / 8
 #pragma unroll
     for (int e = 0; e < RB; ++e) {
@@ -803,6 +806,7 @@ struct DwArgs {
   int T, G, R;
   long long limit;
   int drop;
+  int after_expand;                                    // the launch before it is the expand, not the shrink
 };
 
 // A step is 32 rows of 256 columns: 16 KB of x or dy and RB x 8 KB of the
@@ -860,11 +864,14 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
     store(0, 8 * c, zero8);
     store(1, 8 * c, zero8);
   }
-  if (rp == 0) {                                       // the whole cluster leaves
-    // but the launch does not end before the one that it depends on
+  // The factors come from the shrink.  Behind an expand this launch began after the
+  // shrink's end (the expand's CTAs let it begin, one of them at least after its own
+  // wait for the shrink), and shares the SMs with the expand; it only has to end
+  // after it.
+  auto wait_last = [&]() {
     if (blockIdx.x == 0 && blockIdx.y == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
-    return;
-  }
+  };
+  if (rp == 0) return wait_last();                     // the whole cluster leaves
 
   const int s_all = (r1 - r0 + kRows - 1) / kRows, s_per = (s_all + csize - 1) / csize;
   const int sb = min(s_all, rank * s_per), ns = min(s_all, sb + s_per) - sb;
@@ -946,7 +953,7 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
       }
     };
     load_tok(cur, 0);
-    asm volatile("griddepcontrol.wait;" ::: "memory"); // the factors come from the shrink
+    if (!a.after_expand) asm volatile("griddepcontrol.wait;" ::: "memory");
     Ring<kStages> at;
     for (int s0 = 0; s0 < ns && !a.drop; s0 += 4) {
       load_tok(nxt, s0 + 4);
@@ -1043,8 +1050,8 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(D::kTmemCols) : "memory");
   }
+  wait_last();
 }
-
 template <class K, class A>
 zmoe_status launch(K* kernel, dim3 grid, int threads, int csize, bool dependent, int smem, cudaStream_t stream,
                    const A& args, const char* what) {
@@ -1129,7 +1136,7 @@ zmoe_status launch_grad_tiles(const zmoe_lora_grad_args* p, cudaStream_t stream)
   zmoe_status st = p->R <= 64 ? launch_tiles<1, 1>(a, stream) : launch_tiles<1, 2>(a, stream);
   if (st != ZMOE_OK || !p->da) return st;
   const DwArgs d{{p->x, p->dy}, split, {p->da, p->db}, p->scale, p->rank, p->offsets, p->token_of_row,
-                 {p->H, p->N}, p->T, p->G, p->R, tc::wait_limit(), tc::drop_loads()};
+                 {p->H, p->N}, p->T, p->G, p->R, tc::wait_limit(), tc::drop_loads(), p->dx != nullptr};
   return p->R <= 64 ? launch_dw<1>(d, stream) : launch_dw<2>(d, stream);
 }
 

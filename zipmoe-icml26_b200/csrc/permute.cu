@@ -332,21 +332,30 @@ sort_kernel(const SortArgs a) {
 }
 
 // Every CTA sorts all pairs and copies the rows of its own share of the
-// 16-byte vectors; CTA 0 writes the index outputs.
+// 16-byte vectors; CTA 0 writes the index outputs.  A token's slots are split in as
+// many groups as fill the SMs: one SM stores 64 bytes a cycle, so 8 copies of 1024
+// vectors from one CTA would take 1 us.
 __global__ void __launch_bounds__(kSortThreads)
-sort_gather_kernel(const SortArgs a, const uint4* __restrict__ x, int vec, uint4* __restrict__ xp) {
+sort_gather_kernel(const SortArgs a, const uint4* __restrict__ x, int vec, int groups, int per,
+                   uint4* __restrict__ xp) {
   extern __shared__ int sort_smem_raw[];
   int32_t* rows_s = sort_smem_raw + kSortWarps * a.E + 2 * a.E + 32;
+  const int total = a.T * groups * vec;                // the fused launch is small
+  int i = (int)threadIdx.x < per ? (int)(blockIdx.x * per + threadIdx.x) : total;
+  int q = i / vec, c = i - q * vec, t = q / groups;
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (i < total) v = __ldg(x + t * vec + c);           // in flight while the pairs are sorted
   sort_pairs(a, 0, 1, sort_smem_raw, blockIdx.x == 0, rows_s);
   __syncthreads();
-  const int total = a.T * vec;                         // the fused launch is small
-  for (int i = blockIdx.x * kSortThreads + threadIdx.x; i < total; i += gridDim.x * kSortThreads) {
-    const int t = i / vec, c = i - t * vec;
-    const uint4 v = __ldg(x + i);
-    for (int j = 0; j < a.k; ++j) {
+  while (i < total) {
+    for (int j = q - t * groups; j < a.k; j += groups) {
       const int r = rows_s[t * a.k + j];
       if (r >= 0) xp[(size_t)r * vec + c] = v;
     }
+    i += gridDim.x * per;
+    if (i >= total) break;
+    q = i / vec, c = i - q * vec, t = q / groups;
+    v = __ldg(x + t * vec + c);
   }
 }
 
@@ -448,9 +457,14 @@ zmoe_status launch_permute(const zmoe_permute_args* a, cudaStream_t stream) {
       st = allow_smem<sort_gather_kernel>();
       if (st != ZMOE_OK) return st;
       const size_t smem = sort_smem(a->E) + sizeof(int32_t) * (size_t)a->T * a->k;
-      int blocks = (int)(((size_t)a->T * vec + kSortThreads - 1) / kSortThreads);
+      const int full = kNumSMs * kSortThreads / (a->T * vec);
+      const int groups = full < 1 ? 1 : full < a->k ? full : a->k;
+      const int items = a->T * groups * vec;
+      int per = (items / kNumSMs + 255) / 256 * 256;   // of a CTA at a time
+      per = per < 256 ? 256 : per > kSortThreads ? kSortThreads : per;
+      int blocks = (items + per - 1) / per;
       if (blocks > kNumSMs) blocks = kNumSMs;
-      sort_gather_kernel<<<blocks, kSortThreads, smem, stream>>>(sa, reinterpret_cast<const uint4*>(a->x), vec,
+      sort_gather_kernel<<<blocks, kSortThreads, smem, stream>>>(sa, reinterpret_cast<const uint4*>(a->x), vec, groups, per,
                                                                  reinterpret_cast<uint4*>(a->xp));
       return launch_status("sort_gather_kernel");
     }
