@@ -2,13 +2,14 @@
 // and the adapters, over the C ABI of libzmoe.so.  These calls run once per layer
 // and token step, where the host's time counts: checking ten tensors, allocating
 // outputs and filling an argument structure took 10 to 14 us in Python with
-// ctypes and takes 3 to 5 here.  zmoe/ops.py documents each function.
+// ctypes and takes 2 to 4 here.  zmoe/ops.py documents each function.
 //
 // Bad arguments raise ValueError; a status other than ZMOE_OK raises
 // zmoe._lib.ZmoeError with the library's message.  Work runs on the arguments'
 // device and that device's current torch stream.
 #include <torch/extension.h>
 
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -65,6 +66,11 @@ int to_int(int64_t v, const char* name) {
   return static_cast<int>(v);
 }
 
+// An output, without at::empty's way through the dispatcher (0.3 us each).
+Tensor empty(at::IntArrayRef shape, at::ScalarType type, at::Device device) {
+  return Tensor(at::detail::empty_cuda(shape, type, device, std::nullopt));
+}
+
 py::object* g_error = nullptr;                         // zmoe._lib.ZmoeError
 
 // Calls an entry point with the GIL released.
@@ -103,12 +109,11 @@ py::tuple permute(const Tensor& idx, const OptTensor& x, int64_t E, int64_t capa
   a.capacity = to_int(capacity, "capacity");
   a.seq_len = to_int(seq_len, "seq_len");
   const int64_t rows = std::max<int64_t>(T * k, 1);
-  const auto i32 = idx.options();
-  Tensor counts = at::empty({E}, i32), offsets = at::empty({E + 1}, i32), row_of = at::empty({T, k}, i32),
-         tor = at::empty({rows}, i32);
+  Tensor counts = empty({E}, kI32, dev), offsets = empty({E + 1}, kI32, dev), row_of = empty({T, k}, kI32, dev),
+         tor = empty({rows}, kI32, dev);
   py::object xp = py::none();
   if (x) {
-    Tensor t = at::empty({rows, (int64_t)a.H}, x->options());
+    Tensor t = empty({rows, (int64_t)a.H}, kBF16, dev);
     a.xp = static_cast<uint16_t*>(t.data_ptr());
     xp = py::cast(t);
   }
@@ -132,7 +137,7 @@ Tensor permute_grad(const Tensor& dxp, const Tensor& row_of, const OptTensor& ba
   a.H = to_int(H, "H");
   a.k = to_int(k, "k");
   a.rows = to_int(rows, "rows");
-  Tensor dx = dx_ ? *dx_ : at::empty({T, H}, dxp.options());
+  Tensor dx = dx_ ? *dx_ : empty({T, H}, kBF16, dev);
   a.dx = arg<uint16_t>(dx, "dx", kBF16, {T, H}, dev);
   call("zmoe_permute_grad", dev, [&](zmoe_stream_t s) { return zmoe_permute_grad(&a, s); });
   return dx;
@@ -159,22 +164,22 @@ py::tuple combine_grad(const Tensor& dout, const Tensor& y, const Tensor& row_of
   a.k = to_int(k, "k");
   a.mode = to_int(mode, "mode");
   a.rows = to_int(rows, "rows");
-  Tensor dy = dy_ ? *dy_ : at::empty({rows, H}, y.options()), dw = at::empty({T, k}, w.options());
+  Tensor dy = dy_ ? *dy_ : empty({rows, H}, kBF16, dev), dw = empty({T, k}, kF32, dev);
   a.dy = arg<uint16_t>(dy, "dy", kBF16, {rows, H}, dev);
   a.dtopk_w = static_cast<float*>(dw.data_ptr());
   py::object dysh = py::none(), dg = py::none(), dx = py::none();
   if (y_shared) {
-    Tensor t = at::empty({T, H}, dout.options());
+    Tensor t = empty({T, H}, kBF16, dev);
     a.dy_shared = static_cast<uint16_t*>(t.data_ptr());
     dysh = py::cast(t);
   }
   if (shared_gate) {
-    Tensor t = at::empty({T}, w.options());
+    Tensor t = empty({T}, kF32, dev);
     a.dshared_gate = static_cast<float*>(t.data_ptr());
     dg = py::cast(t);
   }
   if (mode == ZMOE_ROUTE_SWITCH) {
-    Tensor t = at::empty({T, H}, dout.options());
+    Tensor t = empty({T, H}, kBF16, dev);
     a.dx = static_cast<uint16_t*>(t.data_ptr());
     dx = py::cast(t);
   }
@@ -187,7 +192,7 @@ py::tuple lora_plan(const Tensor& adapter, int64_t G) {
   const int64_t T = adapter.size(0);
   const int32_t* ids = arg<int32_t>(adapter, "adapter", kI32, {T}, dev);
   const int g = to_int(G, "G"), t = to_int(T, "T");
-  Tensor offsets = at::empty({std::max<int64_t>(G, 0) + 1}, adapter.options()), tor = at::empty({T}, adapter.options());
+  Tensor offsets = empty({std::max<int64_t>(G, 0) + 1}, kI32, dev), tor = empty({T}, kI32, dev);
   auto* po = static_cast<int32_t*>(offsets.data_ptr());
   auto* pt = static_cast<int32_t*>(tor.data_ptr());
   call("zmoe_lora_plan", dev, [&](zmoe_stream_t s) { return zmoe_lora_plan(ids, t, g, po, pt, s); });
@@ -224,10 +229,10 @@ Tensor lora(const Tensor& x, const OptTensor& base, const Tensor& a, const Tenso
   p.x = arg<uint16_t>(x, "x", kBF16, {T, (int64_t)p.H}, dev);
   p.base = arg<uint16_t>(base, "base", kBF16, {T, (int64_t)p.N}, dev);
   p.u = arg<float>(u, "u", kF32, {T, (int64_t)p.R}, dev);
-  Tensor out = out_ ? *out_ : at::empty({T, (int64_t)p.N}, x.options()), scratch;
+  Tensor out = out_ ? *out_ : empty({T, (int64_t)p.N}, kBF16, dev), scratch;
   p.out = arg<uint16_t>(out, "out", kBF16, {T, (int64_t)p.N}, dev);
   if (T > ZMOE_LORA_ROWS) {
-    scratch = at::empty({T, (int64_t)p.R}, x.options().dtype(kF32));
+    scratch = empty({T, (int64_t)p.R}, kF32, dev);
     p.scratch = static_cast<float*>(scratch.data_ptr());
   }
   call("zmoe_lora", dev, [&](zmoe_stream_t s) { return zmoe_lora(&p, s); });
@@ -245,9 +250,10 @@ py::tuple lora_grad(const Tensor& dy, const Tensor& x, const Tensor& u, const Te
   p.x = arg<uint16_t>(x, "x", kBF16, {T, (int64_t)p.H}, dev);
   p.u = arg<float>(u, "u", kF32, {T, (int64_t)p.R}, dev);
   p.base = arg<uint16_t>(base, "base", kBF16, {T, (int64_t)p.H}, dev);
-  Tensor dx = dx_ ? *dx_ : at::empty({T, (int64_t)p.H}, dy.options());
+  Tensor dx = dx_ ? *dx_ : empty({T, (int64_t)p.H}, kBF16, dev);
   p.dx = arg<uint16_t>(dx, "dx", kBF16, {T, (int64_t)p.H}, dev);
-  Tensor da = at::empty_like(a), db = at::empty_like(b), scratch = at::empty({T, 2 * (int64_t)p.R}, u.options());
+  Tensor da = empty(a.sizes(), kBF16, dev), db = empty(b.sizes(), kBF16, dev),
+         scratch = empty({T, 2 * (int64_t)p.R}, kF32, dev);
   p.da = static_cast<uint16_t*>(da.data_ptr());
   p.db = static_cast<uint16_t*>(db.data_ptr());
   p.scratch = static_cast<float*>(scratch.data_ptr());

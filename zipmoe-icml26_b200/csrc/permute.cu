@@ -144,8 +144,8 @@ constexpr int kSortCluster = 16;      // the steps are bound by instruction issu
                                       // pairs took 19 us on 8 SMs, 12 on 16
 constexpr int kFusedPairs = 2048;     // pairs every CTA of the fused launch sorts for itself
                                       // (64 experts, rows of 2048, us, fused against two launches: 64 pairs of 4 a
-                                      // token 5.6 and 6.4, of 8 a token 6.7 and 6.4; 2048 pairs 7.7 and 9.0, 8.7 and
-                                      // 8.7; 4096 pairs 12.9 and 12.8, 12.9 and 12.3; 8192 pairs 21.5 and 19.6)
+                                      // token 4.8 and 5.9, of 8 a token 4.6 and 6.4; 2048 pairs 7.7 and 8.6, 7.7 and
+                                      // 8.5; 4096 pairs 12.9 and 11.8, 12.3 and 11.9; 8192 pairs 21.5 and 19.1)
 constexpr int kHold = 16;             // steps of a warp whose pairs stay in registers between the two walks
 constexpr unsigned kFull = 0xffffffffu;
 
