@@ -142,10 +142,10 @@ constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortE = 1024;          // experts: one per thread in the scan, 128 KB of warp counts
 constexpr int kSortCluster = 16;      // the steps are bound by instruction issue: 98 thousand
                                       // pairs took 19 us on 8 SMs, 12 on 16
-constexpr int kFusedPairs = 2048;     // pairs every CTA of the fused launch sorts for itself
+constexpr int kFusedPairs = 1024;     // pairs every CTA of the fused launch sorts for itself
                                       // (64 experts, rows of 2048, us, fused against two launches: 64 pairs of 4 a
-                                      // token 4.8 and 5.9, of 8 a token 4.6 and 6.4; 2048 pairs 7.7 and 8.6, 7.7 and
-                                      // 8.5; 4096 pairs 12.9 and 11.8, 12.3 and 11.9; 8192 pairs 21.5 and 19.1)
+                                      // token 4.8 and 6.1, of 8 a token 4.6 and 6.1; 1024 pairs 5.6 and 6.7; 2048 pairs
+                                      // 7.7 and 7.7, at rows of 1024 7.2 and 6.9, of 4096 10.0 and 9.2)
 constexpr int kHold = 16;             // steps of a warp whose pairs stay in registers between the two walks
 constexpr unsigned kFull = 0xffffffffu;
 
@@ -250,7 +250,7 @@ __device__ void sort_pairs(const SortArgs& a, int rank, int csize, int* smem, bo
     if (csize > 1) {
       int n[kSortCluster];
 #pragma unroll
-      for (int c = 0; c < kSortCluster; ++c) n[c] = *cg::this_cluster().map_shared_rank(tot + e1, c);
+      for (int c = 0; c < kSortCluster; ++c) n[c] = c < csize ? *cg::this_cluster().map_shared_rank(tot + e1, c) : 0;
 #pragma unroll
       for (int c = 0; c < kSortCluster; ++c) {
         if (c < rank) before += n[c];
@@ -403,8 +403,9 @@ gather_rows_kernel(const uint4* __restrict__ src, const int32_t* __restrict__ in
   }
 }
 
-// One cluster: a single CTA while its warps hold their pairs, else the largest
-// size.
+// One CTA while each of its warps has one step at most, else the largest cluster
+// (64 groups, one against 16 CTAs, us: 512 pairs 4.9 and 5.4, 1024 pairs 5.6 and
+// 6.2, 2048 pairs 6.9 and 6.3, 16384 pairs 25 and 6.4; 8 CTAs 7.7, 4 CTAs 10.2).
 zmoe_status launch_sort(const SortArgs& a, cudaStream_t stream) {
   const size_t smem = sort_smem(a.E);
   zmoe_status st = allow_smem<sort_kernel>();
@@ -418,7 +419,7 @@ zmoe_status launch_sort(const SortArgs& a, cudaStream_t stream) {
   }
   const int tp = 32 / a.k, steps = (a.T + tp - 1) / tp;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(steps <= kHold * kSortWarps ? 1 : kSortCluster);
+  cfg.gridDim = dim3(steps <= kSortWarps ? 1 : kSortCluster);
   cfg.blockDim = dim3(kSortThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
