@@ -195,3 +195,43 @@ def test_empty_batches():
     assert (ops.combine_grad(torch.ones(3, 16, dtype=torch.bfloat16).cuda(), z, row, torch.ones(3, 2).cuda(), 0)[1] == 0).all()
     counts, offsets, *_ = ops.permute(row, torch.ones(3, 16, dtype=torch.bfloat16).cuda(), 4)
     assert (counts == 0).all() and (offsets == 0).all()
+
+
+# lists of 131072 pairs and more: full and ragged last CTAs, one expert, as many as there may be
+@pytest.mark.parametrize("T,k,E", [(131072, 1, 1), (131073, 1, 3), (32768, 4, 60), (43692, 3, 700), (17001, 8, 1024), (4229, 31, 896),
+                                   (4096, 32, 1024)])
+@pytest.mark.parametrize("bad", [False, True])
+def test_sort_of_many_pairs(T, k, E, bad):
+    ops = _ops()
+    k_e = min(k, E)
+    idx = np.full((T, k), -1, np.int32)
+    idx[:, :k_e] = _idx(T, k_e, E, T, bad)
+    offs, tor, row_of = _plain_rows(idx, E)
+    x = torch.randn(T, 8, generator=torch.Generator().manual_seed(T)).to(torch.bfloat16)
+    for xd in (x.cuda(), None):
+        counts, offsets, r_of, t_of, xp = ops.permute(torch.from_numpy(idx).cuda(), xd, E)
+        assert np.array_equal(counts.cpu().numpy(), np.diff(offs))
+        assert np.array_equal(offsets.cpu().numpy(), offs)
+        assert np.array_equal(r_of.cpu().numpy(), row_of)
+        assert np.array_equal(t_of[:len(tor)].cpu().numpy(), tor)
+        if xd is not None:
+            assert torch.equal(xp[:len(tor)].cpu(), x[torch.from_numpy(tor).long()])
+
+
+def test_sort_of_many_pairs_leaves_rows_behind_the_last():
+    from zmoe._lib import PermuteArgs, check, lib
+    import ctypes
+    T, k, E, H = 80000, 2, 60, 8
+    idx = torch.full((T, k), -1, dtype=torch.int32)
+    idx[::100, 1] = 7
+    n = T // 100
+    d, x = idx.cuda(), torch.ones(T, H, dtype=torch.bfloat16).cuda()
+    counts, offsets = torch.empty(E, dtype=torch.int32).cuda(), torch.empty(E + 1, dtype=torch.int32).cuda()
+    row_of, tor = torch.empty(T, k, dtype=torch.int32).cuda(), torch.full((T * k,), -7, dtype=torch.int32).cuda()
+    xp = torch.full((T * k, H), 5.0, dtype=torch.bfloat16).cuda()
+    a = PermuteArgs(topk_idx=d.data_ptr(), x=x.data_ptr(), T=T, H=H, E=E, k=k, counts=counts.data_ptr(), offsets=offsets.data_ptr(),
+                    row_of=row_of.data_ptr(), token_of_row=tor.data_ptr(), xp=xp.data_ptr())
+    check(lib.zmoe_permute(ctypes.byref(a), torch.cuda.current_stream().cuda_stream), "zmoe_permute")
+    assert tor[:n].tolist() == list(range(0, T, 100)) and (tor[n:] == -7).all()
+    assert (xp[:n] == 1).all() and (xp[n:] == 5).all()
+    assert int(counts.sum()) == n and int(counts[7]) == n

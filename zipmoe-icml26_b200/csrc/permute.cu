@@ -20,7 +20,9 @@
 //     itself and copies its own share of the rows, so that nothing waits on
 //     another CTA;
 //   * more: one cluster sorts, and the copy follows as a dependent launch that
-//     loads x while the sort finishes.
+//     loads x while the sort finishes;
+//   * from kWidePairs on: CTAs of an ordinary launch count their shares, one CTA
+//     turns the counts into first rows, and the CTAs place their pairs.
 //
 // With a capacity (Switch) drops depend on the rank within a sequence, and
 // three small launches do it: (1) one CTA per expert ranks its tokens in token
@@ -146,6 +148,9 @@ constexpr int kFusedPairs = 1024;     // pairs every CTA of the fused launch sor
                                       // (64 experts, rows of 2048, us, fused against two launches: 64 pairs of 4 a
                                       // token 4.8 and 6.1, of 8 a token 4.6 and 6.1; 1024 pairs 5.6 and 6.7; 2048 pairs
                                       // 7.7 and 7.7, at rows of 1024 7.2 and 6.9, of 4096 10.0 and 9.2)
+constexpr int kWidePairs = 131072;    // pairs from which the sort takes three launches of kWideCtas CTAs instead of
+constexpr int kWideCtas = 64;         // one cluster (with the copy of rows of 2048, us: 65536 pairs 73.8 and 70.8, 98 thousand
+                                      // 87.3 and 87.2, 393 thousand 313 and 357; 128 CTAs 312).  All launches fit the SMs together
 constexpr int kHold = 16;             // steps of a warp whose pairs stay in registers between the two walks
 constexpr unsigned kFull = 0xffffffffu;
 
@@ -157,12 +162,22 @@ struct SortArgs {
   int32_t* offsets;                   // [E + 1]; with rest the first E entries
   int32_t* row_of;                    // [T, k] or nullptr
   int32_t* token_of_row;              // [T * k] or nullptr: the copy of the rows writes it
+  int wide;                           // sort in three launches: steps per warp; else 0
 };
+
+// The wide sort's CTAs: all but the last keep their counts, and then their first
+// rows, in row_of at their own first token, where they are the only ones to write
+// in the end; the last one keeps its counts in the output `counts`.
+__device__ __forceinline__ int32_t* wide_counts(const SortArgs& a, int cta, int ctas) {
+  return cta == ctas - 1 ? a.counts : a.row_of + (size_t)cta * kSortWarps * a.wide * (32 / a.k) * a.k;
+}
 
 // Sorts the pairs of tokens [0, T) by expert over the CTAs of a cluster (rank
 // of csize).  smem: hist [kSortWarps][E], tot [E], base [E], warp_sums.
 // write: this CTA writes the outputs in global memory.  rows_s (or nullptr)
 // receives every pair's row in shared memory.
+// kWide: the CTA is one of an ordinary launch: 1 writes its counts, 2 reads its first rows.
+template <int kWide>
 __device__ void sort_pairs(const SortArgs& a, int rank, int csize, int* smem, bool write, int32_t* rows_s) {
   int* hist = smem;
   int* tot = hist + kSortWarps * a.E;
@@ -173,7 +188,7 @@ __device__ void sort_pairs(const SortArgs& a, int rank, int csize, int* smem, bo
   const int tp = 32 / k;                               // whole tokens per step of a warp
   const int nw = kSortWarps * csize;
   const int steps_all = (a.T + tp - 1) / tp;
-  const int per = (steps_all + nw - 1) / nw;           // steps per warp
+  const int per = kWide ? a.wide : (steps_all + nw - 1) / nw;   // steps per warp
   const int s0 = min(steps_all, (rank * kSortWarps + warp) * per), s1 = min(steps_all, s0 + per);
   const int jl = lane % k, tl = lane / k;              // slot and token of this lane in a step
   const bool used = tl < tp;
@@ -240,51 +255,64 @@ __device__ void sort_pairs(const SortArgs& a, int rank, int csize, int* smem, bo
       hist[w * E + e] = run;
       run += n;
     }
-    tot[e] = run;
+    if (kWide == 1) wide_counts(a, rank, csize)[e] = run;
+    else tot[e] = run;
   }
-  if (csize > 1) cg::this_cluster().sync();
-  else __syncthreads();
-  int all = 0, before = 0;
+  if (kWide == 1) return;
   const int e1 = threadIdx.x;
-  if (e1 < E) {
-    if (csize > 1) {
-      int n[kSortCluster];
-#pragma unroll
-      for (int c = 0; c < kSortCluster; ++c) n[c] = c < csize ? *cg::this_cluster().map_shared_rank(tot + e1, c) : 0;
-#pragma unroll
-      for (int c = 0; c < kSortCluster; ++c) {
-        if (c < rank) before += n[c];
-        all += n[c];
-      }
-    } else {
-      all = tot[e1];
+  if (kWide == 2) {
+    asm volatile("griddepcontrol.wait;" ::: "memory"); // the counts have become first rows
+    if (e1 < E) {
+      const bool last = rank == csize - 1;             // its rows end an expert's
+      const int32_t* p = last ? a.offsets + e1 + 1 : wide_counts(a, rank, csize) + e1;
+      int n;
+      asm volatile("ld.global.cg.b32 %0, [%1];" : "=r"(n) : "l"(p) : "memory");
+      base[e1] = last ? n - tot[e1] : n;
     }
-  }
-  int incl = all;
+  } else {
+    if (csize > 1) cg::this_cluster().sync();
+    else __syncthreads();
+    int all = 0, before = 0;
+    if (e1 < E) {
+      if (csize > 1) {
+        int n[kSortCluster];
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int o = __shfl_up_sync(kFull, incl, d);
-    if (lane >= d) incl += o;
-  }
-  if (lane == 31) warp_sums[warp] = incl;
-  __syncthreads();
-  if (warp == 0) {
-    int v = warp_sums[lane], si = v;
+        for (int c = 0; c < kSortCluster; ++c) n[c] = c < csize ? *cg::this_cluster().map_shared_rank(tot + e1, c) : 0;
+#pragma unroll
+        for (int c = 0; c < kSortCluster; ++c) {
+          if (c < rank) before += n[c];
+          all += n[c];
+        }
+      } else {
+        all = tot[e1];
+      }
+    }
+    int incl = all;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int o = __shfl_up_sync(kFull, si, d);
-      if (lane >= d) si += o;
+      const int o = __shfl_up_sync(kFull, incl, d);
+      if (lane >= d) incl += o;
     }
-    warp_sums[lane] = si - v;
-  }
-  __syncthreads();
-  if (e1 < E) {
-    const int first = warp_sums[warp] + incl - all;
-    base[e1] = first + before;
-    if (write && rank == 0) {
-      if (a.counts) a.counts[e1] = all;
-      a.offsets[e1] = first;
-      if (e1 == E - 1 && !a.rest) a.offsets[E] = first + all;
+    if (lane == 31) warp_sums[warp] = incl;
+    __syncthreads();
+    if (warp == 0) {
+      int v = warp_sums[lane], si = v;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(kFull, si, d);
+        if (lane >= d) si += o;
+      }
+      warp_sums[lane] = si - v;
+    }
+    __syncthreads();
+    if (e1 < E) {
+      const int first = warp_sums[warp] + incl - all;
+      base[e1] = first + before;
+      if (write && rank == 0) {
+        if (a.counts) a.counts[e1] = all;
+        a.offsets[e1] = first;
+        if (e1 == E - 1 && !a.rest) a.offsets[E] = first + all;
+      }
     }
   }
   __syncthreads();
@@ -325,10 +353,91 @@ sort_kernel(const SortArgs a) {
   extern __shared__ int sort_smem_raw[];
   cg::cluster_group cl = cg::this_cluster();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the copy may load x meanwhile
-  sort_pairs(a, (int)cl.block_rank(), (int)cl.num_blocks(), sort_smem_raw, true, nullptr);
+  sort_pairs<0>(a, (int)cl.block_rank(), (int)cl.num_blocks(), sort_smem_raw, true, nullptr);
   // the last remote reads happened before the base scan's barriers of each
   // CTA; wait for the cluster so that no CTA leaves while its totals are read
   cl.sync();
+}
+
+// Many pairs: CTAs count their shares, one CTA turns the counts into first rows, and
+// the CTAs count again (beside the first two launches) and place their pairs.
+__global__ void __launch_bounds__(kSortThreads)
+sort_count_kernel(const SortArgs a) {
+  extern __shared__ int sort_smem_raw[];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  sort_pairs<1>(a, (int)blockIdx.x, (int)gridDim.x, sort_smem_raw, true, nullptr);
+}
+
+__global__ void __launch_bounds__(kSortThreads)
+sort_place_kernel(const SortArgs a) {
+  extern __shared__ int sort_smem_raw[];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  sort_pairs<2>(a, (int)blockIdx.x, (int)gridDim.x, sort_smem_raw, true, nullptr);
+}
+
+// counts of (CTA, expert) -> first rows.  1024 / E groups of threads take runs of
+// CTAs; a thread holds its run's counts of one expert.
+__global__ void __launch_bounds__(kSortThreads)
+sort_first_kernel(const SortArgs a, int ctas) {
+  __shared__ int sums[kSortThreads], warp_sums[32];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int E = a.E, groups = kSortThreads / E, g = threadIdx.x / E, e = threadIdx.x % E;
+  const int run = (ctas + groups - 1) / groups, c0 = min(ctas, g * run), c1 = g < groups ? min(ctas, c0 + run) : c0;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  int n = 0;
+#pragma unroll 8
+  for (int c = c0; c < c1; ++c) {
+    int v;
+    asm volatile("ld.global.cg.b32 %0, [%1];" : "=r"(v) : "l"(wide_counts(a, c, ctas) + e));
+    n += v;
+  }
+  if (g < groups) sums[threadIdx.x] = n;
+  __syncthreads();
+  int all = 0, before = 0;
+  for (int q = 0; q < groups; ++q) {
+    const int v = g < groups ? sums[q * E + e] : 0;
+    if (q < g) before += v;
+    all += v;
+  }
+  // experts' first rows: a scan over the threads of group 0
+  int incl = g == 0 ? all : 0;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(kFull, incl, d);
+    if (lane >= d) incl += o;
+  }
+  if (lane == 31) warp_sums[warp] = incl;
+  __syncthreads();
+  if (warp == 0) {
+    const int v = warp_sums[lane];
+    int si = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(kFull, si, d);
+      if (lane >= d) si += o;
+    }
+    warp_sums[lane] = si - v;
+  }
+  __syncthreads();
+  if (g == 0) {
+    const int first = warp_sums[warp] + incl - all;
+    a.offsets[e] = first;
+    if (e == E - 1) a.offsets[E] = first + all;
+    sums[e] = first;                                   // sums have been read
+  }
+  __syncthreads();
+  if (g < groups) {
+    int at = sums[e] + before;
+#pragma unroll 8
+    for (int c = c0; c < c1; ++c) {
+      int32_t* p = wide_counts(a, c, ctas) + e;
+      int v;
+      asm volatile("ld.global.cg.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+      *p = c == ctas - 1 ? all : at;                   // the last CTA's place is the output `counts`
+      at += v;
+    }
+  }
 }
 
 // Every CTA sorts all pairs and copies the rows of its own share of the
@@ -345,7 +454,7 @@ sort_gather_kernel(const SortArgs a, const uint4* __restrict__ x, int vec, int g
   int q = i / vec, c = i - q * vec, t = q / groups;
   uint4 v = make_uint4(0, 0, 0, 0);
   if (i < total) v = __ldg(x + t * vec + c);           // in flight while the pairs are sorted
-  sort_pairs(a, 0, 1, sort_smem_raw, blockIdx.x == 0, rows_s);
+  sort_pairs<0>(a, 0, 1, sort_smem_raw, blockIdx.x == 0, rows_s);
   __syncthreads();
   while (i < total) {
     for (int j = q - t * groups; j < a.k; j += groups) {
@@ -377,7 +486,7 @@ scatter_rows_kernel(const uint4* __restrict__ x, int T, int vec, int k, const in
   for (int j0 = 0; j0 < k; j0 += 4) {
     int r[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {                      // asm: not before the wait, not from a read-only cache
+    for (int j = 0; j < 4; ++j) {                      // asm: stays behind the wait
       r[j] = -1;
       if (j0 + j < k) asm volatile("ld.global.b32 %0, [%1];" : "=r"(r[j]) : "l"(row_of + t * k + j0 + j) : "memory");
     }
@@ -401,6 +510,35 @@ gather_rows_kernel(const uint4* __restrict__ src, const int32_t* __restrict__ in
     const int c = (int)(i % vec);
     dst[r * vec + c] = __ldg(src + (size_t)__ldg(index + r) * vec + c);
   }
+}
+
+// A launch that may begin when the CTAs of the one before it say so.
+template <class... P, class... Q>
+zmoe_status launch_dependent(const char* what, void (*kernel)(P...), int ctas, size_t smem, cudaStream_t stream, Q... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  ZMOE_CUDA_RET(cudaLaunchKernelEx(&cfg, kernel, args...));
+  return launch_status(what);
+}
+
+zmoe_status launch_sort_wide(const SortArgs& a, int ctas, cudaStream_t stream) {
+  zmoe_status st = allow_smem<sort_count_kernel>();
+  if (st == ZMOE_OK) st = allow_smem<sort_place_kernel>();
+  if (st != ZMOE_OK) return st;
+  const size_t smem = sort_smem(a.E);
+  sort_count_kernel<<<ctas, kSortThreads, smem, stream>>>(a);
+  st = launch_status("sort_count_kernel");
+  if (st == ZMOE_OK) st = launch_dependent("sort_first_kernel", sort_first_kernel, 1, 0, stream, a, ctas);
+  if (st == ZMOE_OK) st = launch_dependent("sort_place_kernel", sort_place_kernel, ctas, smem, stream, a);
+  return st;
 }
 
 // One CTA while each of its warps has one step at most, else the largest cluster
@@ -453,7 +591,7 @@ zmoe_status launch_permute(const zmoe_permute_args* a, cudaStream_t stream) {
   zmoe_status st;
   bool copies_tokens = false;
   if (a->capacity <= 0 && a->E <= kSortE && a->k <= 32) {
-    SortArgs sa{a->topk_idx, a->T, a->k, a->E, 0, a->counts, a->offsets, a->row_of, a->token_of_row};
+    SortArgs sa{a->topk_idx, a->T, a->k, a->E, 0, a->counts, a->offsets, a->row_of, a->token_of_row, 0};
     if (a->xp && a->T * a->k <= kFusedPairs && vec > 0 && (long long)a->T * vec < 1 << 30) {
       st = allow_smem<sort_gather_kernel>();
       if (st != ZMOE_OK) return st;
@@ -470,7 +608,14 @@ zmoe_status launch_permute(const zmoe_permute_args* a, cudaStream_t stream) {
       return launch_status("sort_gather_kernel");
     }
     if (a->xp && vec > 0) sa.token_of_row = nullptr;
-    st = launch_sort(sa, stream);
+    const int tp = 32 / a->k, steps = (a->T + tp - 1) / tp;
+    const int per = (steps + kWideCtas * kSortWarps - 1) / (kWideCtas * kSortWarps);
+    if (a->T * a->k >= kWidePairs && kSortWarps * per * tp * a->k >= a->E) {
+      sa.wide = per;
+      st = launch_sort_wide(sa, (steps + kSortWarps * per - 1) / (kSortWarps * per), stream);
+    } else {
+      st = launch_sort(sa, stream);
+    }
     copies_tokens = true;
   } else {
     ZMOE_CUDA_RET(cudaMemsetAsync(a->row_of, 0xff, sizeof(int32_t) * (size_t)a->T * a->k, stream));
@@ -508,7 +653,7 @@ zmoe_status launch_lora_plan(const int32_t* adapter, int T, int G, int32_t* offs
     ZMOE_CUDA_RET(cudaMemsetAsync(offsets, 0, sizeof(int32_t) * (size_t)(G + 1), stream));
     return ZMOE_OK;
   }
-  return launch_sort(SortArgs{adapter, T, 1, G + 1, 1, nullptr, offsets, nullptr, token_of_row}, stream);
+  return launch_sort(SortArgs{adapter, T, 1, G + 1, 1, nullptr, offsets, nullptr, token_of_row, 0}, stream);
 }
 
 zmoe_status launch_gather_rows(const void* src, const int32_t* index, int rows, int row_bytes, void* dst,
