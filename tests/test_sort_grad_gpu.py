@@ -235,3 +235,33 @@ def test_sort_of_many_pairs_leaves_rows_behind_the_last():
     assert tor[:n].tolist() == list(range(0, T, 100)) and (tor[n:] == -7).all()
     assert (xp[:n] == 1).all() and (xp[n:] == 5).all()
     assert int(counts.sum()) == n and int(counts[7]) == n
+
+
+@pytest.mark.parametrize("T", [300, 9000, 70000])
+def test_sort_replayed_and_on_two_streams(T):
+    ops = _ops()
+    k, E, H = 2, 60, 64
+    idx = [torch.from_numpy(_idx(T, k, E, s)).cuda() for s in range(3)]
+    x = torch.randn(T, H, generator=torch.Generator().manual_seed(T)).to(torch.bfloat16).cuda()
+    want = [ops.permute(i, x, E) for i in idx]
+    held = idx[0].clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.permute(held, x, E)
+        total = got[4].float().sum(0)                   # reads the copy right behind it
+    for i, w in zip(idx, want):
+        held.copy_(i)
+        graph.replay()
+        assert all(torch.equal(p, q) for p, q in zip(got, w))
+        assert torch.equal(total, w[4].float().sum(0))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    res = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for j, q in enumerate(streams):
+            with torch.cuda.stream(q):
+                res[j].append(ops.permute(idx[j], x, E))
+    torch.cuda.synchronize()
+    for j in range(2):
+        assert all(torch.equal(p, q) for r in res[j] for p, q in zip(r, want[j]))
