@@ -1099,7 +1099,18 @@ zmoe_status launch_tiles(TileArgs a, cudaStream_t stream) {
   if (st == ZMOE_OK) st = allow_smem<lora_expand_kernel<DIR, RB>>();
   if (st != ZMOE_OK) return st;
   const int c = share(tiles, (a.K1 + kStep - 1) / kStep, kNumSMs * S::kPerSM, 2, 8, 8, true);
-  a.parts = share(tiles, (a.K2 + kStep - 1) / kStep, kNumSMs * E::kPerSM, 5, 5, 64, false);
+  const int steps2 = (a.K2 + kStep - 1) / kStep;
+  if (a.u_in) {
+    // dA and dB want the other half of the SMs: about one CTA an SM, of four steps at
+    // least (us with the forward's rule and with this one: 16380 rows of 60 adapters,
+    // 3 parts and 1, 82 and 77; 2047 rows of one, 16 parts and 9, 30.1 and 27.1; 64
+    // rows of 12, 24 parts and 6, 20.8 and 16.7)
+    a.parts = (kNumSMs + tiles / 2) / tiles;
+    a.parts = a.parts > steps2 / 4 ? steps2 / 4 : a.parts;
+    a.parts = a.parts < 1 ? 1 : a.parts;
+  } else {
+    a.parts = share(tiles, steps2, kNumSMs * E::kPerSM, 5, 5, 64, false);
+  }
   ZMOE_CHECK_ARG(units * c < (1LL << 31) && units * a.parts < (1LL << 31), "lora: T=%d rows are too many for one launch",
                  a.T);
   st = launch(lora_shrink_kernel<DIR, RB>, dim3((unsigned)(units * c)), S::kThreads, c, false, S::kSmem, stream, a,
@@ -1116,7 +1127,16 @@ zmoe_status launch_dw(const DwArgs& a, cudaStream_t stream) {
   if (st != ZMOE_OK) return st;
   const int tiles = (a.M[0] + D::kCols - 1) / D::kCols + (a.M[1] + D::kCols - 1) / D::kCols;
   const int steps = (a.T + Dw<RB>::kRows - 1) / Dw<RB>::kRows;
-  const int csize = share((long long)tiles * a.G, (steps + a.G - 1) / a.G, kNumSMs * Dw<RB>::kPerSM, 2, 8, 8, true);
+  const long long units = (long long)tiles * a.G;
+  const int most = steps / a.G / 5;
+  // One adapter: as many CTAs as there are SMs.  Several have uneven rows: up to 4 CTAs
+  // a tile while they are not far too many, so that the longest does not end alone.
+  // Five steps each at least.
+  // (us: 2047 rows of one, 30 tiles x 4 CTAs 27.1, x 8 31.8; 8192 rows of 4, 64 tiles x
+  // 2 58.7, x 4 47.8; 65536 rows of 16, 256 tiles x 2 286, x 4 255, x 8 260; 32768 rows
+  // of 60 experts, 840 tiles x 1 121, x 2 139)
+  int csize = 1;
+  while (csize < 8 && csize * 2 <= most && units * csize * 2 <= (a.G > 1 && csize < 4 ? 8 * kNumSMs : kNumSMs)) csize *= 2;
   return launch(lora_dw_kernel<RB>, dim3((unsigned)(tiles * csize), (unsigned)a.G), kDwThreads, csize, true,
                 Dw<RB>::kSmem, stream, a, "lora_dw_kernel");
 }
