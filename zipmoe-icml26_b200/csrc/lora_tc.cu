@@ -613,6 +613,8 @@ __global__ void __launch_bounds__(Expand<RB>::kThreads, Expand<RB>::kPerSM) lora
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // dA's and dB's CTAs may come as SMs free up; TMEM is this CTA's by now
+  if (DIR == 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = tmem_slot;
   auto free_tmem = [&]() {
     // the launch does not end before the shrink has, whatever its CTAs had to do
@@ -686,10 +688,6 @@ __global__ void __launch_bounds__(Expand<RB>::kThreads, Expand<RB>::kPerSM) lora
     const int ahead = min(nc, kStages);
     for (int s = 0; s < ahead && !a.drop; ++s) step();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (DIR == 1 && l == 0) {                          // the shrink has ended: dA and dB may begin
-      __threadfence();
-      asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    }
     const int n8 = min(rp, R) / 8;                     // chunks in memory; zeros behind them up to rp / 8
 #pragma unroll
     for (int e = 0; e < RB; ++e) {
@@ -806,7 +804,6 @@ struct DwArgs {
   int T, G, R;
   long long limit;
   int drop;
-  int after_expand;                                    // the launch before it is the expand, not the shrink
 };
 
 // A step is 32 rows of 256 columns: 16 KB of x or dy and RB x 8 KB of the
@@ -864,10 +861,7 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
     store(0, 8 * c, zero8);
     store(1, 8 * c, zero8);
   }
-  // The factors come from the shrink.  Behind an expand this launch began after the
-  // shrink's end (the expand's CTAs let it begin, one of them at least after its own
-  // wait for the shrink), and shares the SMs with the expand; it only has to end
-  // after it.
+  // the launch does not end before the one in front has, whatever its CTAs had to do
   auto wait_last = [&]() {
     if (blockIdx.x == 0 && blockIdx.y == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
   };
@@ -953,7 +947,7 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
       }
     };
     load_tok(cur, 0);
-    if (!a.after_expand) asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // the factors are the shrink's
     Ring<kStages> at;
     for (int s0 = 0; s0 < ns && !a.drop; s0 += 4) {
       load_tok(nxt, s0 + 4);
@@ -1156,7 +1150,7 @@ zmoe_status launch_grad_tiles(const zmoe_lora_grad_args* p, cudaStream_t stream)
   zmoe_status st = p->R <= 64 ? launch_tiles<1, 1>(a, stream) : launch_tiles<1, 2>(a, stream);
   if (st != ZMOE_OK || !p->da) return st;
   const DwArgs d{{p->x, p->dy}, split, {p->da, p->db}, p->scale, p->rank, p->offsets, p->token_of_row,
-                 {p->H, p->N}, p->T, p->G, p->R, tc::wait_limit(), tc::drop_loads(), p->dx != nullptr};
+                 {p->H, p->N}, p->T, p->G, p->R, tc::wait_limit(), tc::drop_loads()};
   return p->R <= 64 ? launch_dw<1>(d, stream) : launch_dw<2>(d, stream);
 }
 
