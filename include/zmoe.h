@@ -348,7 +348,7 @@ typedef struct zmoe_lora_grad_args {
   uint16_t* dx;               /* [T, H] BF16 out or NULL */
   uint16_t* da;               /* [G, R, H] BF16 out or NULL */
   uint16_t* db;               /* [G, N, R] BF16 out or NULL */
-  float* scratch;             /* [T, 2 R] fp32 */
+  float* scratch;             /* [T, R] fp32 */
 } zmoe_lora_grad_args;
 
 zmoe_status zmoe_lora_grad(const zmoe_lora_grad_args* a, zmoe_stream_t stream);

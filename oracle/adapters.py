@@ -10,7 +10,7 @@ import torch
 
 F64 = torch.float64
 STEP = 2.0 ** -23
-SPLIT = 2.0 ** -16            # an fp32 factor carried as two BF16 values: each rounds by 2^-8 at most
+SPLIT = 2.0 ** -16            # what adding up the products of an fp32 factor's BF16 terms (three, exact) may add
 
 
 def permute_grad(dxp, row_of, base=None):

@@ -31,7 +31,7 @@ constexpr int kRows = 8;                               // the matrix instruction
 constexpr int kCluster = 8;                            // at most
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxR = ZMOE_LORA_MAX_RANK;
-constexpr int kPitch = kMaxR + 8;                      // BF16 of a row of u: 16-byte rows on different banks
+constexpr int kPitch = kMaxR + 32;                     // BF16 of a row of u: two rows' 64 bytes on different banks
 
 __device__ __forceinline__ void mma16n8k16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                            uint32_t b1) {
@@ -65,7 +65,7 @@ lora_rows_kernel(const zmoe_lora_args a) {
   __shared__ Unit unit_s;
   __shared__ float part[8 * kRows * 16];               // [parts of the slice][kRows][ranks]
   __shared__ float up[kRows * kMaxR];                  // the CTA's sums, read by the cluster
-  __shared__ __align__(16) uint16_t us[2][kRows * kPitch];   // s u, high and low halves
+  __shared__ __align__(16) uint16_t us[3][kRows * kPitch];   // s u, in three terms
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), csize = (int)cl.num_blocks();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = lane >> 2, quad = lane & 3;
@@ -135,7 +135,7 @@ lora_rows_kernel(const zmoe_lora_args a) {
     pp[(2 * quad) * 16 * mt + 8] = d[2];
     pp[(2 * quad + 1) * 16 * mt + 8] = d[3];
   }
-  for (int i = tid; i < kRows * kPitch; i += kThreads) us[0][i] = us[1][i] = 0;
+  for (int i = tid; i < kRows * kPitch; i += kThreads) us[0][i] = us[1][i] = us[2][i] = 0;
   // ---- this warp's first tiles of B's rows, while the cluster meets -----------------------
   // A tile is 16 output columns: a lane's 16 bytes of rows l / 4 and l / 4 + 8 per
   // 32 ranks, and base at its four results (two columns, two tokens).
@@ -148,7 +148,7 @@ lora_rows_kernel(const zmoe_lora_args a) {
     uint4 lo[KB], hi[KB];
     uint16_t base[4];
   };
-  constexpr int kPre = 8 / KB;
+  constexpr int kPre = 4 / KB;                         // with s u in registers, as many as fit
   TileRegs pre[kPre];
   auto load_tile = [&](int tile, TileRegs& w) {
     const int n = n0 + 16 * tile + row;
@@ -186,39 +186,46 @@ lora_rows_kernel(const zmoe_lora_args a) {
     if (r >= rk) s = 0.0f;
     if (rank == 0 && a.u) a.u[(size_t)un.row0 * R + i] = s;
     s *= scale;
-    // two BF16 values carry s to 2^-16; an infinite first has no remainder
-    const float high = round_bf16(s);
-    us[0][m * kPitch + r] = f32_to_bf16_bits(high);
-    us[1][m * kPitch + r] = f32_to_bf16_bits(fabsf(high) <= 3.4e38f ? s - high : 0.0f);
+    uint32_t t[3];
+    split(s, t);
+#pragma unroll
+    for (int q = 0; q < 3; ++q) us[q][m * kPitch + r] = (uint16_t)(t[q] >> 16);
   }
   cl.barrier_arrive();                                 // partial sums stay until every CTA has read them
   __syncthreads();
+  // s u of this lane, the same for every tile of B.  (Read again for each tile, its
+  // three terms made shared memory the bound: 96 requests 22.4 us against 18.2.)
+  uint4 uf[KB][3];
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int q = 0; q < 3; ++q) uf[kb][q] = *reinterpret_cast<const uint4*>(&us[q][row * kPitch + 32 * kb + 8 * quad]);
   // ---- this CTA's slice of N --------------------------------------------------------------
   for (int t0 = warp; t0 < tiles; t0 += kWarps * kPre) {
 #pragma unroll
     for (int j = 0; j < kPre; ++j) {
       const int tile = t0 + kWarps * j;
       if (tile >= tiles) break;
-      float d[4] = {0.f, 0.f, 0.f, 0.f};
+      float d[2][4] = {};                              // sums of the first term and of the others
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {                // columns from the rank on may hold anything
+        const int k = 32 * kb + 8 * quad;
+        if (k < rk && k + 8 > rk) {
+          pre[j].lo[kb] = keep(pre[j].lo[kb], rk - k);
+          pre[j].hi[kb] = keep(pre[j].hi[kb], rk - k);
+        }
+      }
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
         if (kb >= k32) break;
-        const int k = 32 * kb + 8 * quad;
-        const uint4 hi = *reinterpret_cast<const uint4*>(&us[0][row * kPitch + k]);
-        const uint4 lo = *reinterpret_cast<const uint4*>(&us[1][row * kPitch + k]);
-        uint4 wl = pre[j].lo[kb], wh = pre[j].hi[kb];
-        if (k < rk && k + 8 > rk) {                    // columns from the rank on may hold anything
-          wl = keep(wl, rk - k);
-          wh = keep(wh, rk - k);
-        }
-        mma32(d, wl, wh, hi);
-        mma32(d, wl, wh, lo);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) mma32(d[q > 0], pre[j].lo[kb], pre[j].hi[kb], uf[kb][q]);
       }
       const int n = n0 + 16 * tile + row;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {                    // rows n and n + 8, the lane's two tokens
         const int t = t2[c & 1], nn = n + 8 * (c >> 1);
-        if (t >= 0 && nn < n1) a.out[(size_t)t * N + nn] = f32_to_bf16_bits(bf16_bits_to_f32(pre[j].base[c]) + d[c]);
+        if (t >= 0 && nn < n1) a.out[(size_t)t * N + nn] = f32_to_bf16_bits(bf16_bits_to_f32(pre[j].base[c]) + (d[0][c] + d[1][c]));
       }
       if (tile + kWarps * kPre < tiles) load_tile(tile + kWarps * kPre, pre[j]);
     }

@@ -82,5 +82,32 @@ __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
   }
 }
 
+// A value as three BF16 terms (the upper halves of t) whose sum it is: each is what
+// the ones before leave, cut to 8 bits.  Infinities and NaN are their first term.
+__device__ __forceinline__ void split(float f, uint32_t (&t)[3]) {
+  const uint32_t b = __float_as_uint(f);
+  const bool finite = (b & 0x7f800000u) != 0x7f800000u;
+  const float rest = finite ? f - __uint_as_float(b & 0xffff0000u) : 0.0f;
+  t[0] = finite || !(b & 0x007fffffu) ? b : b | 0x00400000u;   // a NaN stays one
+  t[1] = __float_as_uint(rest);
+  t[2] = __float_as_uint(rest - __uint_as_float(t[1] & 0xffff0000u));
+}
+
+// Eight values as three vectors of BF16 terms.
+__device__ __forceinline__ void split8(const float4 (&f)[2], uint4 (&t)[3]) {
+  const float v[8] = {f[0].x, f[0].y, f[0].z, f[0].w, f[1].x, f[1].y, f[1].z, f[1].w};
+  uint32_t w[3][4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t a[3], b[3];
+    split(v[2 * q], a);
+    split(v[2 * q + 1], b);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) w[i][q] = __byte_perm(a[i], b[i], 0x7632);
+  }
+#pragma unroll
+  for (int i = 0; i < 3; ++i) t[i] = make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]);
+}
+
 }  // namespace lora
 }  // namespace zmoe

@@ -18,11 +18,12 @@
 // for 2047 rows of 2048 in and 5632 out at rank 16: tiles of whole rows leave SMs
 // without work.)
 //
-// Precision: x, dy, A and B are BF16 as given.  u and v are fp32 sums; as
-// operands of the second product they are carried as two BF16 values each
-// (hi = bf16(u), lo = bf16(u - hi)), an error of 2^-16 instead of 2^-8: the
-// second product costs twice the MMAs, which HBM hides, and the output has one
-// visible rounding.
+// Precision: x, dy, A and B are BF16 as given.  u and v are fp32 sums, and enter
+// the second product whole: as three BF16 terms of 8 bits each whose sum they are.
+// That costs three times the MMAs, which HBM hides, and the output has one
+// rounding.  (Two terms, 16 bits, saved MMAs and a third of the operand's shared
+// memory, but moved the outputs four times as far from an fp32 product's as the order
+// of its sums does.)
 //
 // Warps have roles: some load, one issues the MMAs, some drain TMEM.  Operands
 // come in by cp.async (rows are gathered by token, 16 bytes a lane) into
@@ -83,6 +84,12 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
+__device__ __forceinline__ void arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void st16(uint32_t dst, const uint4& v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
 __device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void prefetch(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -100,6 +107,18 @@ __device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t adesc, uint64_t
       : "memory");
 }
 
+// The same with A in TMEM.
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                       uint32_t accumulate, uint32_t go) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(go)
+      : "memory");
+}
+
 // One lane of a converged warp.
 __device__ __forceinline__ uint32_t elect_one() {
   uint32_t go;
@@ -111,15 +130,25 @@ __device__ __forceinline__ uint32_t elect_one() {
   return go;
 }
 
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&f)[8]) {
-  uint32_t r[8];
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&f)[8]) {
+  uint32_t r[8];
+  tmem_ld8(taddr, r);
   tmem_wait_ld();
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(r[i]);
 }
+
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint4& v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(v.x), "r"(v.y), "r"(v.z),
+               "r"(v.w)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // 32 columns, 16 at a time, one wait.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&lo)[16], uint32_t (&hi)[16]) {
@@ -202,20 +231,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Eight fp32 values as two BF16 vectors, f = hi + lo up to 2^-16; an infinite
-// hi has no remainder.
-__device__ __forceinline__ void split8(const float (&f)[8], uint4& hi, uint4& lo) {
-  uint32_t h[4], l[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    h[q] = pack2(f[2 * q], f[2 * q + 1]);
-    const float b0 = __uint_as_float(h[q] << 16), b1 = __uint_as_float(h[q] & 0xffff0000u);
-    l[q] = pack2(fabsf(b0) <= 3.4e38f ? f[2 * q] - b0 : 0.0f, fabsf(b1) <= 3.4e38f ? f[2 * q + 1] - b1 : 0.0f);
-  }
-  hi = make_uint4(h[0], h[1], h[2], h[3]);
-  lo = make_uint4(l[0], l[1], l[2], l[3]);
-}
-
 struct TileArgs {
   const uint16_t* src;                                 // shrink: [T, K1]
   const uint16_t* w1;                                  // DIR 0: A [G, R, K1]; DIR 1: B [G, K1, R]
@@ -226,8 +241,8 @@ struct TileArgs {
   int T, K1, K2, G, R;
   uint16_t* out;                                       // [T, K2]
   float* u;                                            // DIR 0: [T, R] out or nullptr
-  const float* u_in;                                   // DIR 1: the forward pass's u, [T, R], or nullptr
-  uint16_t* split;                                     // DIR 0: [T][s u hi, lo][R]; DIR 1: [T][v hi, lo, u hi, lo][R]
+  float* second;                                       // factor of the second product, [T, R]: s u, or v
+  int weights;                                         // DIR 1: dA and dB are wanted too
   int parts;                                           // expand: CTAs per tile
   long long limit;                                     // of a wait, in clock64 cycles
   int drop;                                            // error-path test: the loaders load nothing
@@ -465,14 +480,7 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
   float4* part = reinterpret_cast<float4*>(smem);      // [rp / 4][kTile][4], in the ring's place
   const bool mine = m < un.rows && warp < kMmaWarp;
   const size_t grow = (size_t)(un.row0 + m);
-  auto load_u = [&](int i, float4 (&u)[2]) {           // the forward pass's u at this row's columns 8 i on
-    if (DIR == 1 && a.u_in && mine && 8 * i < min(rp, R)) {
-      const float4* up = reinterpret_cast<const float4*>(a.u_in + grow * R + 8 * i);
-      u[0] = __ldg(up);
-      u[1] = __ldg(up + 1);
-    }
-  };
-  auto write = [&](int i, float (&f)[8], const float4 (&u)[2]) {
+  auto write = [&](int i, float (&f)[8]) {
     const int c0 = 8 * i;
     if (!mine || c0 >= R) return;
 #pragma unroll
@@ -485,35 +493,19 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] *= scale;
-    uint4 hi, lo;
-    split8(f, hi, lo);
-    uint16_t* sp = a.split + grow * (DIR ? 4 : 2) * R + c0;
-    *reinterpret_cast<uint4*>(sp) = hi;
-    *reinterpret_cast<uint4*>(sp + R) = lo;
-    if (DIR == 1 && a.u_in) {
-      float w[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (c0 + e >= rk) w[e] = 0.0f;
-      split8(w, hi, lo);
-      *reinterpret_cast<uint4*>(sp + 2 * R) = hi;
-      *reinterpret_cast<uint4*>(sp + 3 * R) = lo;
-    }
+    float4* sp = reinterpret_cast<float4*>(a.second + grow * R + c0);
+    sp[0] = make_float4(f[0], f[1], f[2], f[3]);
+    sp[1] = make_float4(f[4], f[5], f[6], f[7]);
   };
   const int first = csize == 1 ? half : rank + csize * half, stride = 2 * csize;
-  float4 u[2];
-  if (warp < kMmaWarp) {
-    load_u(first, u);
-    wait_bar(smem_u32(&sums), 0, guard);             // every MMA has read the ring
-  }
+  if (warp < kMmaWarp) wait_bar(smem_u32(&sums), 0, guard);   // every MMA has read the ring
   tc_fence_after();
   if (csize == 1) {
     if (warp < kMmaWarp)
       for (int i = first; i < n8; i += stride) {
         float f[8];
         tmem_ld8(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(8 * i), f);
-        if (i != first) load_u(i, u);
-        write(i, f, u);
+        write(i, f);
       }
   } else {
     if (warp < kMmaWarp)
@@ -544,8 +536,7 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
             f[4] += v[c][1].x; f[5] += v[c][1].y; f[6] += v[c][1].z; f[7] += v[c][1].w;
           }
         }
-        if (i != first) load_u(i, u);
-        write(i, f, u);
+        write(i, f);
       }
     cl.barrier_arrive();                               // partial sums stay until every CTA has read them
   }
@@ -565,19 +556,21 @@ template <int RB>
 struct Expand {
   static constexpr uint32_t kStageBytes = kXBytes + RB * 8192;
   static constexpr int kPerSM = RB == 1 ? 2 : 1;
-  static constexpr int kStages = RB == 1 ? 3 : 4;
-  static constexpr uint32_t kOperand = RB * 2 * 16384; // hi blocks, lo blocks
-  static constexpr int kOuts = 4;                      // 64-column outputs in TMEM
+  static constexpr int kStages = RB == 1 ? 4 : 6;      // 96 KB / 192 KB
+  // TMEM: outputs of 64 columns, then the operand's terms, two BF16 a column
+  static constexpr int kOuts = RB == 1 ? 2 : 4;
+  static constexpr uint32_t kOperand = 64 * kOuts, kTerm = 32 * RB;
+  static constexpr uint32_t kTmemCols = RB == 1 ? 256 : 512;
   static constexpr int kDrainWarps = 8;                // two groups, taking steps in turn
   static constexpr int kThreads = 32 * (kDrainWarps + 1 + kLoadWarps);
-  static constexpr int kSmem = 1024 + kStages * kStageBytes + kOperand;
+  static constexpr int kSmem = 1024 + kStages * kStageBytes;
 };
 
 template <int DIR, int RB>
 __global__ void __launch_bounds__(Expand<RB>::kThreads, Expand<RB>::kPerSM) lora_expand_kernel(const TileArgs a) {
   using L = Expand<RB>;
   constexpr int kStages = L::kStages, kDrainWarps = L::kDrainWarps, kOuts = L::kOuts;
-  constexpr uint32_t kTmemCols = 64 * kOuts;
+  constexpr uint32_t kTmemCols = L::kTmemCols;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[kStages], used[kStages], operand, out_full[kOuts], out_free[kOuts], last;
   __shared__ uint32_t tmem_slot;
@@ -595,7 +588,7 @@ __global__ void __launch_bounds__(Expand<RB>::kThreads, Expand<RB>::kPerSM) lora
         mbar_init(&full[s], kLoaders);
         mbar_init(&used[s], kDrainWarps / 2);
       }
-      mbar_init(&operand, kLoaders);
+      mbar_init(&operand, 32 * kDrainWarps);
       mbar_init(&last, 1);
       for (int i = 0; i < kOuts; ++i) {
         mbar_init(&out_full[i], 1);
@@ -668,7 +661,6 @@ __global__ void __launch_bounds__(Expand<RB>::kThreads, Expand<RB>::kPerSM) lora
   const int rp = (rk + 15) & ~15;                      // the MMAs' K
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t ring = smem_u32(smem), full_a = smem_u32(full), used_a = smem_u32(used);
-  const uint32_t op = ring + kStages * L::kStageBytes;
 
   if (warp > kDrainWarps) {
     // ------------------------------------------------------------------ load
@@ -684,26 +676,9 @@ __global__ void __launch_bounds__(Expand<RB>::kThreads, Expand<RB>::kPerSM) lora
       cp_arrive(full_a + 8 * at.slot);
       at.next();
     };
-    // base and weights do not depend on the shrink: they go first
+    // base and weights do not depend on the shrink, and do not wait for it
     const int ahead = min(nc, kStages);
     for (int s = 0; s < ahead && !a.drop; ++s) step();
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int n8 = min(rp, R) / 8;                     // chunks in memory; zeros behind them up to rp / 8
-#pragma unroll
-    for (int e = 0; e < RB; ++e) {
-      const int c = (l & 7) + 8 * e;
-      if (c < rp / 8 && !a.drop) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int m = (l >> 3) + 16 * j;
-          const uint16_t* sp = a.split + (size_t)(un.row0 + min(m, un.rows - 1)) * (DIR ? 4 : 2) * R + 8 * c;
-          const int bytes = c < n8 ? 16 : 0;
-          cp16(op + xo + 2048u * j + 16384u * e, bytes ? sp : a.split, bytes);
-          cp16(op + xo + 2048u * j + 16384u * (e + RB), bytes ? sp + R : a.split, bytes);
-        }
-      }
-    }
-    if (!a.drop) cp_arrive(smem_u32(&operand));
     for (int s = ahead; s < nc && !a.drop; ++s) {
       wait_bar(used_a + 8 * at.slot, at.parity ^ 1u, guard);
       step();
@@ -713,10 +688,10 @@ __global__ void __launch_bounds__(Expand<RB>::kThreads, Expand<RB>::kPerSM) lora
     // ------------------------------------------------------------------ MMAs
     const uint32_t go = elect_one(), id = idesc(kStep, 0, DIR);
     Ring<kStages> at;
-    const uint64_t du = smem_desc(op);
     const uint64_t dw0 = DIR ? desc_mn(ring + kXBytes, 8192) : smem_desc(ring + kXBytes);
     const uint32_t of = smem_u32(out_full), fr = smem_u32(out_free);
     wait_bar(smem_u32(&operand), 0, guard);
+    tc_fence_after();
 #pragma unroll 1
     for (int o = 0; o < nc; ++o) {
       const int buf = o % kOuts;
@@ -729,21 +704,52 @@ __global__ void __launch_bounds__(Expand<RB>::kThreads, Expand<RB>::kPerSM) lora
       const uint64_t dw = dw0 + at.slot * (L::kStageBytes >> 4);
       const uint32_t d = tmem + 64 * (uint32_t)buf;
 #pragma unroll 1
-      for (int kk = 0; 16 * kk < rp; ++kk) {
-        const uint64_t db = dw + (DIR ? (2048 >> 4) * kk : (kk >> 2) * (8192 >> 4) + 2 * (kk & 3));
-        const uint64_t da = du + (kk >> 2) * (16384 >> 4) + 2 * (kk & 3);
-        mma_ss(d, da, db, id, kk != 0, go);
-        mma_ss(d, da + RB * (16384 >> 4), db, id, 1, go);
-      }
+      for (int term = 2; term >= 0; --term)            // the small terms first: their sums lose nothing
+#pragma unroll 1
+        for (int kk = 0; 16 * kk < rp; ++kk)
+          mma_ts(d, tmem + L::kOperand + term * L::kTerm + 8 * kk,
+                 dw + (DIR ? (2048 >> 4) * kk : (kk >> 2) * (8192 >> 4) + 2 * (kk & 3)), id, term != 2 || kk != 0, go);
       commit_at(of + 8 * buf, go);
       at.next();
     }
     finish_mmas(&last, go, a.limit);
   } else {
+    // ------------------------------------------------------------------ operand
+    // The first product's sums of this lane's row, every other eight columns, in three
+    // BF16 terms.  They were written beside this launch's beginning: loads past L1.
+    const int m = q * 32 + lane;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    {
+      const int c_end = rp / 8, c_in = min(rp, R) / 8; // zeros between them
+      const float4* p = reinterpret_cast<const float4*>(a.second + (size_t)(un.row0 + min(m, un.rows - 1)) * R);
+      float4 v[4 * RB][2];
+#pragma unroll
+      for (int e = 0; e < 4 * RB; ++e) {
+        const int c = half + 2 * e;
+        v[e][0] = v[e][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c < c_in) {
+          v[e][0] = __ldcg(p + 2 * c);
+          v[e][1] = __ldcg(p + 2 * c + 1);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4 * RB; ++e) {
+        const int c = half + 2 * e;
+        if (c < c_end) {
+          uint4 t[3];
+          split8(v[e], t);
+#pragma unroll
+          for (int i = 0; i < 3; ++i)
+            tmem_st4(tmem + ((uint32_t)(q * 32) << 16) + L::kOperand + i * L::kTerm + 4 * (uint32_t)c, t[i]);
+        }
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&operand);
+    }
     // ------------------------------------------------------------------ outputs
     // base (in the ring) plus product, one rounding.  The two groups of four
     // warps take alternate steps, so that one's latencies hide behind the other's
-    const int m = q * 32 + lane;
     const uint32_t ro = place(q * 32 + (lane >> 3), lane & 7, 0), mo = place(m, 0, 0);
     Ring<kStages> at;
     if (half) at.next();
@@ -796,7 +802,7 @@ __global__ void __launch_bounds__(Expand<RB>::kThreads, Expand<RB>::kPerSM) lora
 // ---------------------------------------------------------------------------
 struct DwArgs {
   const uint16_t* src[2];                              // x [T, H], dy [T, N]
-  const uint16_t* split;                               // [T][v hi, v lo, u hi, u lo][R]
+  const float* factor[2];                              // v, u: [T, R]
   uint16_t* out[2];                                    // da [G, R, H], db [G, N, R]
   const float* scale;
   const int32_t *rank, *offsets, *token_of_row;
@@ -806,28 +812,35 @@ struct DwArgs {
   int drop;
 };
 
-// A step is 32 rows of 256 columns: 16 KB of x or dy and RB x 8 KB of the
-// factor's two halves.  (With 128 columns the factor is read twice as often and
+// A step is 32 rows of 256 columns: 16 KB of x or dy and RB x 12 KB of the
+// factor's three terms.  (With 128 columns the factor is read twice as often and
 // there are twice as many CTAs to set up: 39 against 36 us for 60 groups of
 // 273 rows, 2048 and 1408 columns, rank 32; 13.3 against 14.9 us for one group
 // of 2047 rows.)
-template <int RB>
+// kWide: R <= 32, the terms lie side by side as the columns of one product (3 R), so that
+// an MMA reads the 128 columns of x or dy once for all of them; else a term has RB blocks
+// of 64 columns (R <= 64 RB), and the terms' products are added one by one.
+template <int RB, bool kWide>
 struct Dw {
   static constexpr int kRows = 32, kCols = 2 * kTile;
   static constexpr uint32_t kBlock = kRows * 128;      // 64 columns
-  static constexpr uint32_t kSrcBytes = kRows * kCols * 2, kHalf = RB * kBlock;
-  static constexpr uint32_t kStageBytes = kSrcBytes + 2 * kHalf;
+  static constexpr uint32_t kSrcBytes = kRows * kCols * 2;
+  static constexpr uint32_t kStageBytes = kSrcBytes + (kWide ? 2 : 3 * RB) * kBlock;
   static constexpr int kPerSM = RB == 1 ? 2 : 1;
-  static constexpr int kStages = RB == 1 ? 4 : 6;      // 96 KB / 192 KB
-  static constexpr uint32_t kTmemCols = 2 * RB * 64;
+  static constexpr int kStages = kWide ? 4 : RB == 1 ? 3 : 5;   // 96 / 84 / 200 KB
+  static constexpr int kDepth = kWide ? 4 : 3;         // steps of the factor in registers
+  static constexpr uint32_t kTileCols = kWide ? 96 : RB * 64;   // of TMEM, for 128 columns of x or dy
+  static constexpr uint32_t kTmemCols = kWide ? 256 : 2 * kTileCols;
   static constexpr int kSmem = 1024 + kStages * kStageBytes;
 };
 
-constexpr int kDwThreads = kLoaders + 32;              // four warps load and then drain, one issues the MMAs
+// Four warps load x or dy and then drain, one issues the MMAs, four load and split the
+// factor: in the first four it would hold up the copies of later steps.
+constexpr int kDwThreads = 2 * kLoaders + 32;
 
-template <int RB>
-__global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(const DwArgs a) {
-  using D = Dw<RB>;
+template <int RB, bool kWide>
+__global__ void __launch_bounds__(kDwThreads, Dw<RB, kWide>::kPerSM) lora_dw_kernel(const DwArgs a) {
+  using D = Dw<RB, kWide>;
   constexpr int kStages = D::kStages, kRows = D::kRows;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[kStages], used[kStages], sums, last;
@@ -874,7 +887,7 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
   const uint32_t ring = smem_u32(smem), full_a = smem_u32(full), used_a = smem_u32(used);
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&full[s], kLoaders);
+      mbar_init(&full[s], 2 * kLoaders);               // copies, and the factor's stores
       mbar_init(&used[s], 1);
     }
     mbar_init(&sums, 1);
@@ -898,7 +911,7 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
     // ------------------------------------------------------------------ MMAs
     {
       const uint32_t go = elect_one();
-      const uint32_t id = idesc(rp, 1, 1);
+      const uint32_t id = idesc(kWide ? 3 * rp : rp, 1, 1);
       const uint64_t dx0 = desc_mn(ring, D::kBlock), dw0 = desc_mn(ring + D::kSrcBytes, D::kBlock);
       Ring<kStages> at;
 #pragma unroll 1
@@ -912,8 +925,9 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
             const uint64_t da = dx0 + off + kk * (2048 >> 4) + n * (2 * D::kBlock >> 4);
-            mma_ss(tmem + n * RB * 64, da, dw, id, (s | kk) != 0, go);
-            mma_ss(tmem + n * RB * 64, da, dw + (D::kHalf >> 4), id, 1, go);
+#pragma unroll
+            for (int i = kWide ? 0 : 2; i >= 0; --i)
+              mma_ss(tmem + n * D::kTileCols, da, dw + i * (RB * D::kBlock >> 4), id, (!kWide && i != 2) || (s | kk) != 0, go);
           }
         }
         commit_at(used_a + 8 * at.slot, go);
@@ -923,17 +937,74 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
       finish_mmas(&last, go, a.limit);
     }
     __syncwarp();
+  } else if (warp > kLoadWarps) {
+    // ------------------------------------------------------------------ factor
+    // Pieces of eight columns of a row, kDepth steps ahead in fp32 (a step waits a load's
+    // latency / kDepth) and past L1, as the shrink may run beside this launch's beginning.
+    constexpr int kPieces = kWide ? 1 : 2 * RB, kDepth = D::kDepth;
+    const int l = tid - 32 * (kLoadWarps + 1);
+    const int n8 = min(rp, R) / 8;                     // chunks in memory; zeros behind them up to rp / 8
+    int row[kPieces], chunk[kPieces];
+    uint32_t at3[kPieces][3];                          // the terms' places; 0: not a piece
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int sh = !kWide ? 3 : rp > 16 ? 2 : 1;     // kWide: 2 or 4 chunks a row
+      row[i] = (l >> sh) + 16 * (i & 1);
+      chunk[i] = (l & ((1 << sh) - 1)) + 8 * (i >> 1);
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+        at3[i][q] = row[i] < kRows && chunk[i] < rp / 8
+                        ? D::kSrcBytes + place(row[i], kWide ? q * (rp / 8) + chunk[i] : 8 * RB * q + chunk[i], D::kBlock)
+                        : 0u;
+    }
+    const float* factor = a.factor[which];
+    float4 held[kDepth][kPieces][2];
+    auto load = [&](float4 (&h)[kPieces][2], int s) {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int r = r0 + (sb + s) * kRows + row[i];
+        h[i][0] = h[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (s < ns && r < r1 && row[i] < kRows && chunk[i] < n8) {
+          const float4* p = reinterpret_cast<const float4*>(factor + (size_t)r * R + 8 * chunk[i]);
+          h[i][0] = __ldcg(p);
+          h[i][1] = __ldcg(p + 1);
+        }
+      }
+    };
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // v is the shrink's
+#pragma unroll
+    for (int e = 0; e < kDepth; ++e) load(held[e], e);
+    Ring<kStages> at;
+    for (int s0 = 0; s0 < ns && !a.drop; s0 += kDepth) {
+#pragma unroll
+      for (int e = 0; e < kDepth; ++e) {
+        const int s = s0 + e;
+        if (s >= ns) break;
+        if (s >= kStages) wait_bar(used_a + 8 * at.slot, at.parity ^ 1u, guard);
+        const uint32_t st = ring + at.slot * D::kStageBytes;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+          if (at3[i][0]) {
+            uint4 t[3];
+            split8(held[e][i], t);
+#pragma unroll
+            for (int q = 0; q < 3; ++q) st16(st + at3[i][q], t[q]);
+          }
+        }
+        arrive_at(full_a + 8 * at.slot);               // (the MMA warp's fence covers the stores)
+        load(held[e], s + kDepth);
+        at.next();
+      }
+    }
   } else {
     // ------------------------------------------------------------------ loaders
     // 32 rows x 256 columns of src per step: this thread's chunk (its lane) of rows
-    // warp + 4j; the factor's two halves: rows tid/8 + 16j, chunk tid%8 (+ 8)
-    const int col = m0 + 8 * lane, fr = tid >> 3, fc = tid & 7;
-    uint32_t xo[2], fo = D::kSrcBytes + place(fr, fc, 0);
+    // warp + 4j
+    const int col = m0 + 8 * lane;
+    uint32_t xo[2];
     xo[0] = place(warp, lane, D::kBlock);              // + 1024 every eight rows
     xo[1] = place(warp + 4, lane, D::kBlock);
     const uint16_t* src = a.src[which];
-    const int n8 = min(rp, R) / 8;                     // chunks in memory; zeros behind them up to rp / 8
-    const uint16_t* fp = a.split + ((size_t)(r0 + sb * kRows + fr) * 4 + 2 * which) * R + 8 * fc;
     const int first = r0 + sb * kRows;
     const int xbytes = col < M ? 16 : 0;
     const uint16_t* xsrc = xbytes ? src + col : src;
@@ -947,7 +1018,6 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
       }
     };
     load_tok(cur, 0);
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // the factors are the shrink's
     Ring<kStages> at;
     for (int s0 = 0; s0 < ns && !a.drop; s0 += 4) {
       load_tok(nxt, s0 + 4);
@@ -957,28 +1027,12 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
         if (s >= ns) break;
         if (s >= kStages) wait_bar(used_a + 8 * at.slot, at.parity ^ 1u, guard);
         const uint32_t st = ring + at.slot * D::kStageBytes;
-        const int row = first + s * kRows;
 #pragma unroll
         for (int j = 0; j < kRows / 4; ++j) {
           const int t = __shfl_sync(kFull, cur[e], warp + 4 * j);
           const bool in = (unsigned)t < (unsigned)a.T;
           cp16(st + xo[j & 1] + 1024u * (j >> 1), in ? xsrc + (size_t)(unsigned)t * (unsigned)M : src, in ? xbytes : 0);
         }
-#pragma unroll
-        for (int i = 0; i < RB; ++i) {
-          const int c = fc + 8 * i;
-          if (c < rp / 8) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const int bytes = row + fr + 16 * j < r1 && c < n8 ? 16 : 0;
-              const uint16_t* p = bytes ? fp + (size_t)(64 * j) * R + 64 * i : a.split;   // 16 rows of 4 R
-              const uint32_t o = st + fo + (uint32_t)(i * kRows * 128 + j * 2048);
-              cp16(o, p, bytes);
-              cp16(o + D::kHalf, bytes ? p + R : p, bytes);
-            }
-          }
-        }
-        fp += (size_t)kRows * 4 * R;
         cp_arrive(full_a + 8 * at.slot);
         at.next();
       }
@@ -997,7 +1051,19 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB>::kPerSM) lora_dw_kernel(con
     for (int c = 0; c < 2 * n8; ++c) {                 // tile c / n8, rank columns 8 (c % n8) on
       const int t = c >= n8, c8 = 8 * (c - t * n8);
       float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (ns > 0) tmem_ld8(tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(t * RB * 64 + c8), v);
+      if (ns > 0) {
+        const uint32_t at = tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(t * D::kTileCols + c8);
+        if (kWide) {
+          uint32_t w[3][8];
+#pragma unroll
+          for (int q = 0; q < 3; ++q) tmem_ld8(at + q * rp, w[q]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(w[0][e]) + (__uint_as_float(w[1][e]) + __uint_as_float(w[2][e]));
+        } else {
+          tmem_ld8(at, v);
+        }
+      }
       if (csize > 1) {
         part[(2 * c) * kTile + tid] = make_float4(v[0], v[1], v[2], v[3]);
         part[(2 * c + 1) * kTile + tid] = make_float4(v[4], v[5], v[6], v[7]);
@@ -1094,7 +1160,7 @@ zmoe_status launch_tiles(TileArgs a, cudaStream_t stream) {
   if (st != ZMOE_OK) return st;
   const int c = share(tiles, (a.K1 + kStep - 1) / kStep, kNumSMs * S::kPerSM, 2, 8, 8, true);
   const int steps2 = (a.K2 + kStep - 1) / kStep;
-  if (a.u_in) {
+  if (a.weights) {
     // dA and dB want the other half of the SMs: about one CTA an SM, of four steps at
     // least (us with the forward's rule and with this one: 16380 rows of 60 adapters,
     // 3 parts and 1, 82 and 77; 2047 rows of one, 16 parts and 9, 30.1 and 27.1; 64
@@ -1114,13 +1180,13 @@ zmoe_status launch_tiles(TileArgs a, cudaStream_t stream) {
                 "lora_expand_kernel");
 }
 
-template <int RB>
+template <int RB, bool kWide>
 zmoe_status launch_dw(const DwArgs& a, cudaStream_t stream) {
-  using D = Dw<RB>;
-  zmoe_status st = allow_smem<lora_dw_kernel<RB>>();
+  using D = Dw<RB, kWide>;
+  zmoe_status st = allow_smem<lora_dw_kernel<RB, kWide>>();
   if (st != ZMOE_OK) return st;
   const int tiles = (a.M[0] + D::kCols - 1) / D::kCols + (a.M[1] + D::kCols - 1) / D::kCols;
-  const int steps = (a.T + Dw<RB>::kRows - 1) / Dw<RB>::kRows;
+  const int steps = (a.T + D::kRows - 1) / D::kRows;
   const long long units = (long long)tiles * a.G;
   const int most = steps / a.G / 5;
   // One adapter: as many CTAs as there are SMs.  Several have uneven rows: up to 4 CTAs
@@ -1131,27 +1197,26 @@ zmoe_status launch_dw(const DwArgs& a, cudaStream_t stream) {
   // of 60 experts, 840 tiles x 1 121, x 2 139)
   int csize = 1;
   while (csize < 8 && csize * 2 <= most && units * csize * 2 <= (a.G > 1 && csize < 4 ? 8 * kNumSMs : kNumSMs)) csize *= 2;
-  return launch(lora_dw_kernel<RB>, dim3((unsigned)(tiles * csize), (unsigned)a.G), kDwThreads, csize, true,
-                Dw<RB>::kSmem, stream, a, "lora_dw_kernel");
+  return launch(lora_dw_kernel<RB, kWide>, dim3((unsigned)(tiles * csize), (unsigned)a.G), kDwThreads, csize, true,
+                D::kSmem, stream, a, "lora_dw_kernel");
 }
 
 }  // namespace
 
 zmoe_status launch_tiles(const zmoe_lora_args* p, cudaStream_t stream) {
   const TileArgs a{p->x, p->a, p->b, p->base, p->scale, p->rank, p->offsets, p->token_of_row, p->T, p->H, p->N, p->G,
-                   p->R, p->out, p->u, nullptr, reinterpret_cast<uint16_t*>(p->scratch), 1, tc::wait_limit(), tc::drop_loads()};
+                   p->R, p->out, p->u, p->scratch, 0, 1, tc::wait_limit(), tc::drop_loads()};
   return p->R <= 64 ? launch_tiles<0, 1>(a, stream) : launch_tiles<0, 2>(a, stream);
 }
 
 zmoe_status launch_grad_tiles(const zmoe_lora_grad_args* p, cudaStream_t stream) {
-  uint16_t* split = reinterpret_cast<uint16_t*>(p->scratch);
   const TileArgs a{p->dy, p->b, p->a, p->base, p->scale, p->rank, p->offsets, p->token_of_row, p->T, p->N, p->H, p->G,
-                   p->R, p->dx, nullptr, p->da ? p->u : nullptr, split, 1, tc::wait_limit(), tc::drop_loads()};
+                   p->R, p->dx, nullptr, p->scratch, p->da != nullptr, 1, tc::wait_limit(), tc::drop_loads()};
   zmoe_status st = p->R <= 64 ? launch_tiles<1, 1>(a, stream) : launch_tiles<1, 2>(a, stream);
   if (st != ZMOE_OK || !p->da) return st;
-  const DwArgs d{{p->x, p->dy}, split, {p->da, p->db}, p->scale, p->rank, p->offsets, p->token_of_row,
+  const DwArgs d{{p->x, p->dy}, {p->scratch, p->u}, {p->da, p->db}, p->scale, p->rank, p->offsets, p->token_of_row,
                  {p->H, p->N}, p->T, p->G, p->R, tc::wait_limit(), tc::drop_loads()};
-  return p->R <= 64 ? launch_dw<1>(d, stream) : launch_dw<2>(d, stream);
+  return p->R <= 32 ? launch_dw<1, true>(d, stream) : p->R <= 64 ? launch_dw<1, false>(d, stream) : launch_dw<2, false>(d, stream);
 }
 
 zmoe_status read_error(int32_t* out, int reset) {

@@ -253,7 +253,7 @@ py::tuple lora_grad(const Tensor& dy, const Tensor& x, const Tensor& u, const Te
   Tensor dx = dx_ ? *dx_ : empty({T, (int64_t)p.H}, kBF16, dev);
   p.dx = arg<uint16_t>(dx, "dx", kBF16, {T, (int64_t)p.H}, dev);
   Tensor da = empty(a.sizes(), kBF16, dev), db = empty(b.sizes(), kBF16, dev),
-         scratch = empty({T, 2 * (int64_t)p.R}, kF32, dev);
+         scratch = empty({T, (int64_t)p.R}, kF32, dev);
   p.da = static_cast<uint16_t*>(da.data_ptr());
   p.db = static_cast<uint16_t*>(db.data_ptr());
   p.scratch = static_cast<float*>(scratch.data_ptr());
