@@ -242,7 +242,7 @@ struct TileArgs {
   uint16_t* out;                                       // [T, K2]
   float* u;                                            // DIR 0: [T, R] out or nullptr
   float* second;                                       // factor of the second product, [T, R]: s u, or v
-  int weights;                                         // DIR 1: dA and dB are wanted too
+  long long weights;                                   // DIR 1: tiles of dB, 0 without
   int parts;                                           // expand: CTAs per tile
   long long limit;                                     // of a wait, in clock64 cycles
   int drop;                                            // error-path test: the loaders load nothing
@@ -849,9 +849,11 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB, kWide>::kPerSM) lora_dw_ker
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), csize = (int)cl.num_blocks();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int tilesA = (a.M[0] + D::kCols - 1) / D::kCols;
-  const int unit = (int)(blockIdx.x / csize), g = blockIdx.y;
-  const int which = unit >= tilesA, m0 = (which ? unit - tilesA : unit) * D::kCols, M = a.M[which];
+  // dB of every adapter first: it reads nothing of the launches in front and runs
+  // beside them; dA waits
+  const int unit = (int)(blockIdx.x / csize), unitsB = (a.M[1] + D::kCols - 1) / D::kCols * a.G;
+  const int which = unit < unitsB, M = a.M[which], tiles = (M + D::kCols - 1) / D::kCols;
+  const int index = which ? unit : unit - unitsB, g = index / tiles, m0 = (index - g * tiles) * D::kCols;
   const int R = a.R, rk = rank_of(a.rank, g, R);
   const int r0 = min(max(a.offsets[g], 0), a.T), r1 = min(max(a.offsets[g + 1], 0), a.T);
   uint16_t* out = a.out[which];
@@ -876,7 +878,7 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB, kWide>::kPerSM) lora_dw_ker
   }
   // the launch does not end before the one in front has, whatever its CTAs had to do
   auto wait_last = [&]() {
-    if (blockIdx.x == 0 && blockIdx.y == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
   };
   if (rp == 0) return wait_last();                     // the whole cluster leaves
 
@@ -971,7 +973,7 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB, kWide>::kPerSM) lora_dw_ker
         }
       }
     };
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // v is the shrink's
+    if (!which) asm volatile("griddepcontrol.wait;" ::: "memory");   // v is the shrink's
 #pragma unroll
     for (int e = 0; e < kDepth; ++e) load(held[e], e);
     Ring<kStages> at;
@@ -1160,11 +1162,11 @@ zmoe_status launch_tiles(TileArgs a, cudaStream_t stream) {
   if (st != ZMOE_OK) return st;
   const int c = share(tiles, (a.K1 + kStep - 1) / kStep, kNumSMs * S::kPerSM, 2, 8, 8, true);
   const int steps2 = (a.K2 + kStep - 1) / kStep;
-  if (a.weights) {
-    // dA and dB want the other half of the SMs: about one CTA an SM, of four steps at
-    // least (us with the forward's rule and with this one: 16380 rows of 60 adapters,
-    // 3 parts and 1, 82 and 77; 2047 rows of one, 16 parts and 9, 30.1 and 27.1; 64
-    // rows of 12, 24 parts and 6, 20.8 and 16.7)
+  if (a.weights >= kNumSMs) {
+    // dB runs beside dx and fills the other half of the SMs: about one CTA an SM, of four
+    // steps at least (us with the forward's rule and with this one: 16380 rows of 60
+    // adapters, 3 parts and 1, 82.8 and 79.5; 2047 rows of one, whose dB is 32 CTAs, 16
+    // parts and 9, 29.2 and 31.5)
     a.parts = (kNumSMs + tiles / 2) / tiles;
     a.parts = a.parts > steps2 / 4 ? steps2 / 4 : a.parts;
     a.parts = a.parts < 1 ? 1 : a.parts;
@@ -1192,12 +1194,13 @@ zmoe_status launch_dw(const DwArgs& a, cudaStream_t stream) {
   // One adapter: as many CTAs as there are SMs.  Several have uneven rows: up to 4 CTAs
   // a tile while they are not far too many, so that the longest does not end alone.
   // Five steps each at least.
-  // (us: 2047 rows of one, 30 tiles x 4 CTAs 27.1, x 8 31.8; 8192 rows of 4, 64 tiles x
-  // 2 58.7, x 4 47.8; 65536 rows of 16, 256 tiles x 2 286, x 4 255, x 8 260; 32768 rows
-  // of 60 experts, 840 tiles x 1 121, x 2 139)
+  // (us: 2047 rows of one, 30 tiles x 4 CTAs 29.2, x 8 29.8; 8192 rows of 4, 64 tiles x
+  // 2 52.9, x 4 46.6; 65536 rows of 16, 256 tiles x 2 260, x 4 244, x 8 265; 32768 rows
+  // of 60 experts, 840 tiles x 1 124, x 2 148.  All with rows in every group: the host
+  // does not know the rows, so a bank of G adapters of which one is used is shared like G.)
   int csize = 1;
   while (csize < 8 && csize * 2 <= most && units * csize * 2 <= (a.G > 1 && csize < 4 ? 8 * kNumSMs : kNumSMs)) csize *= 2;
-  return launch(lora_dw_kernel<RB, kWide>, dim3((unsigned)(tiles * csize), (unsigned)a.G), kDwThreads, csize, true,
+  return launch(lora_dw_kernel<RB, kWide>, dim3((unsigned)(units * csize)), kDwThreads, csize, true,
                 D::kSmem, stream, a, "lora_dw_kernel");
 }
 
@@ -1211,7 +1214,7 @@ zmoe_status launch_tiles(const zmoe_lora_args* p, cudaStream_t stream) {
 
 zmoe_status launch_grad_tiles(const zmoe_lora_grad_args* p, cudaStream_t stream) {
   const TileArgs a{p->dy, p->b, p->a, p->base, p->scale, p->rank, p->offsets, p->token_of_row, p->T, p->N, p->H, p->G,
-                   p->R, p->dx, nullptr, p->scratch, p->da != nullptr, 1, tc::wait_limit(), tc::drop_loads()};
+                   p->R, p->dx, nullptr, p->scratch, p->da ? (long long)p->G * ((p->N + 2 * kTile - 1) / (2 * kTile)) : 0, 1, tc::wait_limit(), tc::drop_loads()};
   zmoe_status st = p->R <= 64 ? launch_tiles<1, 1>(a, stream) : launch_tiles<1, 2>(a, stream);
   if (st != ZMOE_OK || !p->da) return st;
   const DwArgs d{{p->x, p->dy}, {p->scratch, p->u}, {p->da, p->db}, p->scale, p->rank, p->offsets, p->token_of_row,
