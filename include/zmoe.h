@@ -295,9 +295,13 @@ zmoe_status zmoe_combine_grad(const zmoe_combine_grad_args* a, zmoe_stream_t str
  * with base = the shared projection's output.  Rows are grouped by adapter:
  * rows offsets[g] .. offsets[g + 1] belong to adapter g, row r is token
  * token_of_row[r] (NULL: row r is token r, as for zmoe_permute's gathered
- * rows with an adapter per expert), every token in one row.  Rows outside [offsets[0], offsets[G]) use no
- * adapter: out = base.  rank[g] <= R is the rank of adapter g: rows of A_g and columns
- * of B_g from rank[g] on are not used, whatever they hold.
+ * rows with an adapter per expert), every token in one row; an entry outside
+ * [0, T) names none, and its row of u is 0.  Rows outside [offsets[0],
+ * offsets[G]) use no adapter: out = base.  rank[g] <= R is the rank of adapter
+ * g: rows of A_g and columns of B_g from rank[g] on are not used, whatever they
+ * hold.  u and v (below) are fp32 sums and enter their products with all 24
+ * bits; an infinity among the inputs reaches the outputs that depend on it as an
+ * infinity or as a NaN.
  * ------------------------------------------------------------------------ */
 /* Rows of a batch from each token's adapter id: offsets [G + 1] and
  * token_of_row [T], tokens ascending inside an adapter; ids outside [0, G) use

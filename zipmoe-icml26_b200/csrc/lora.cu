@@ -183,7 +183,7 @@ lora_rows_kernel(const zmoe_lora_args a) {
 #pragma unroll
     for (int c = 0; c < kCluster; ++c) s += p[c];
     const int m = i / R, r = i - m * R;
-    if (r >= rk) s = 0.0f;
+    if (r >= rk || token_of(a.token_of_row, un.row0 + m, a.T) < 0) s = 0.0f;   // a row of no token has u = 0
     if (rank == 0 && a.u) a.u[(size_t)un.row0 * R + i] = s;
     s *= scale;
     uint32_t t[3];

@@ -480,12 +480,13 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
   float4* part = reinterpret_cast<float4*>(smem);      // [rp / 4][kTile][4], in the ring's place
   const bool mine = m < un.rows && warp < kMmaWarp;
   const size_t grow = (size_t)(un.row0 + m);
+  const bool named = mine && token_of(a.token_of_row, un.row0 + m, a.T) >= 0;   // a row of no token has u = 0
   auto write = [&](int i, float (&f)[8]) {
     const int c0 = 8 * i;
     if (!mine || c0 >= R) return;
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (c0 + e >= rk) f[e] = 0.0f;
+      if (!named || c0 + e >= rk) f[e] = 0.0f;
     if (DIR == 0 && a.u) {
       float4* up = reinterpret_cast<float4*>(a.u + grow * R + c0);
       up[0] = make_float4(f[0], f[1], f[2], f[3]);
