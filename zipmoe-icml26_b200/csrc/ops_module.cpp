@@ -96,7 +96,8 @@ py::tuple permute(const Tensor& idx, const OptTensor& x, int64_t E, int64_t capa
   zmoe_permute_args a{};
   a.topk_idx = arg<int32_t>(idx, "topk_idx", kI32, {T, k}, dev);
   if (x) {
-    if (!x->is_cuda() || x->dim() != 2 || x->size(0) != T || x->scalar_type() != kBF16 || !x->is_contiguous() || x->device() != dev)
+    // rows behind the last token may be there (a buffer for the largest batch) and are not read
+    if (!x->is_cuda() || x->dim() != 2 || x->size(0) < T || x->scalar_type() != kBF16 || !x->is_contiguous() || x->device() != dev)
       value_error("x: expected a contiguous CUDA BF16 tensor with a row for each token");
     a.x = static_cast<const uint16_t*>(x->data_ptr());
     a.H = to_int(x->size(1), "H");
