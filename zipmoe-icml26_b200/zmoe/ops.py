@@ -12,8 +12,12 @@ import numpy as np
 import torch
 
 from . import _lib
-from . import _ops  # C++ side of the calls whose host time counts (csrc/ops_module.cpp)
-from ._lib import CombineArgs, FfnArgs, RouterArgs, ZmoeChunk, ZmoeEncChunk, check, lib
+from ._lib import CombineArgs, FfnArgs, PermuteArgs, RouterArgs, ZmoeChunk, ZmoeEncChunk, check, lib
+
+try:
+    from . import _ops  # C++ side of the calls whose host time counts (csrc/ops_module.cpp)
+except ImportError as e:  # libzmoe.so alone is built: what was there before _ops works without it
+    _ops, _ops_error = None, e
 
 ROUTE_QWEN, ROUTE_DEEPSEEK, ROUTE_SWITCH = 0, 1, 2
 
@@ -248,7 +252,25 @@ def router(x: torch.Tensor, w: torch.Tensor, k: int, mode: int, bias: Optional[t
 def permute(topk_idx: torch.Tensor, x: Optional[torch.Tensor], E: int, capacity: int = 0, seq_len: int = 0):
     """Returns counts, offsets, row_of, token_of_row, xp.  topk_idx is updated
     in place (-1 for capacity drops)."""
-    return _ops.permute(topk_idx, x, E, capacity, seq_len)
+    if _ops is not None:
+        return _ops.permute(topk_idx, x, E, capacity, seq_len)
+    _need(topk_idx, torch.int32, "topk_idx")
+    T, k = topk_idx.shape
+    if x is not None:
+        _need(x, torch.bfloat16, "x")
+        if x.dim() != 2 or x.shape[0] < T:
+            raise ValueError("x: expected a row for each token")
+    dev = topk_idx.device
+    H = x.shape[1] if x is not None else 0
+    counts = torch.empty(E, dtype=torch.int32, device=dev)
+    offsets = torch.empty(E + 1, dtype=torch.int32, device=dev)
+    row_of = torch.empty(T, k, dtype=torch.int32, device=dev)
+    tor = torch.empty(max(T * k, 1), dtype=torch.int32, device=dev)
+    xp = torch.empty(max(T * k, 1), H, dtype=torch.bfloat16, device=dev) if x is not None else None
+    a = PermuteArgs(topk_idx.data_ptr(), _ptr(x), T, H, E, k, capacity, seq_len, counts.data_ptr(),
+                    offsets.data_ptr(), row_of.data_ptr(), tor.data_ptr(), _ptr(xp))
+    check(lib.zmoe_permute(ctypes.byref(a), _stream()), "zmoe_permute")
+    return counts, offsets, row_of, tor, xp
 
 
 def weight_table(mats: Sequence[Sequence[Optional[torch.Tensor]]], device=None) -> torch.Tensor:
@@ -288,11 +310,17 @@ def combine(y: torch.Tensor, row_of: torch.Tensor, topk_w: torch.Tensor, mode: i
 # ---------------------------------------------------------------------------
 # gradients of permute and combine, low-rank adapters
 # ---------------------------------------------------------------------------
+def _ext():
+    if _ops is None:
+        raise ImportError("zmoe._ops is not built (python setup_zipmoe.py build_ext --inplace)") from _ops_error
+    return _ops
+
+
 def permute_grad(dxp: torch.Tensor, row_of: torch.Tensor, base: Optional[torch.Tensor] = None,
                  dx: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Gradient of permute's gather (zmoe_permute_grad): dx[t] = base[t] + sum_j
     dxp[row_of[t, j]].  base (the gradient from other paths) may be dx itself."""
-    return _ops.permute_grad(dxp, row_of, base, dx)
+    return _ext().permute_grad(dxp, row_of, base, dx)
 
 
 def combine_grad(dout: torch.Tensor, y: torch.Tensor, row_of: torch.Tensor, topk_w: torch.Tensor, mode: int,
@@ -302,14 +330,14 @@ def combine_grad(dout: torch.Tensor, y: torch.Tensor, row_of: torch.Tensor, topk
     dshared_gate, dx; the last three are None without y_shared, without
     shared_gate and outside Switch.  Rows of dy that no slot names are left as
     they were (uninitialised when dy is not given)."""
-    return _ops.combine_grad(dout, y, row_of, topk_w, mode, y_shared, shared_gate, x, dy)
+    return _ext().combine_grad(dout, y, row_of, topk_w, mode, y_shared, shared_gate, x, dy)
 
 
 def lora_plan(adapter: torch.Tensor, G: int):
     """Rows of a batch grouped by adapter (zmoe_lora_plan): adapter[t] in [0, G),
     anything else for a token without one.  Returns offsets [G + 1] and
     token_of_row [T], which serve every projection of the step."""
-    return _ops.lora_plan(adapter, G)
+    return _ext().lora_plan(adapter, G)
 
 
 def lora(x: torch.Tensor, base: Optional[torch.Tensor], a: torch.Tensor, b: torch.Tensor,
@@ -322,7 +350,7 @@ def lora(x: torch.Tensor, base: Optional[torch.Tensor], a: torch.Tensor, b: torc
     offsets and token_of_row come from lora_plan, or offsets from permute when
     x holds its gathered rows (an adapter per expert).  out may be base; base
     None counts as zeros.  u (fp32 [T, R]) receives x a^T for lora_grad."""
-    return _ops.lora(x, base, a, b, scale, offsets, token_of_row, rank, out, u)
+    return _ext().lora(x, base, a, b, scale, offsets, token_of_row, rank, out, u)
 
 
 def lora_grad(dy: torch.Tensor, x: torch.Tensor, u: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
@@ -332,4 +360,4 @@ def lora_grad(dy: torch.Tensor, x: torch.Tensor, u: torch.Tensor, a: torch.Tenso
     """Gradient of lora (zmoe_lora_grad) from its u: returns dx = base + v a, da and
     db.  base (the gradient through the shared projection) may be dx itself;
     the gradient of lora's own base is dy."""
-    return _ops.lora_grad(dy, x, u, a, b, scale, offsets, token_of_row, rank, base, dx)
+    return _ext().lora_grad(dy, x, u, a, b, scale, offsets, token_of_row, rank, base, dx)
