@@ -459,7 +459,7 @@ def run_ep(args):
     import datetime
     import torch.distributed as dist
     from zmoe import codec as zc
-    from zmoe import ep
+    from zmoe import ep, ops
     from zmoe import synthetic as syn
     world, rank, local = dist_env()
     torch.cuda.set_device(local)
@@ -543,9 +543,9 @@ def run_ep(args):
         dec_s = st["decode_ns"] * 1e-9
         launches = max(st["decode_timed_launches"], 1)
         achieved = (st["decode_timed_bytes"] / launches) / (dec_s / launches) / 1e9 if dec_s > 0 else 0.0
-        # per step: router 1, permute 3, gathers 2, shared FFN 2, combine 1 + the engine's own
+        # per step: router 1, permute, gathers 2, shared FFN 2, combine 1 + the engine's own
         # (NCCL's own kernels are not counted)
-        ep_launches = 9 * args.steps
+        ep_launches = (6 + ops.permute_launches(args.tokens, s.topk, s.num_experts, s.hidden)) * args.steps
         line = {
             "metric": METRIC, "value": world * args.tokens / (ms / 1e3), "unit": UNIT, "n_gpus": world,
             "steps": args.steps, "warmup": args.warmup, "ms_per_step": ms, "higher_is_better": True,

@@ -179,6 +179,9 @@ typedef struct zmoe_permute_args {
 } zmoe_permute_args;
 
 zmoe_status zmoe_permute(const zmoe_permute_args* a, zmoe_stream_t stream);
+/* Kernels that zmoe_permute launches for these sizes (0 when T is 0; xp counts as
+ * NULL or not, no other pointer is looked at).  zmoe_layer_stats.launches uses it. */
+int zmoe_permute_launches(const zmoe_permute_args* a);
 
 /* --------------------------------------------------------------------------
  * Grouped expert FFN over the permuted rows.

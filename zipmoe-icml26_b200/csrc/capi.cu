@@ -19,6 +19,7 @@ zmoe_status launch_decode_chunks(const zmoe_chunk*, int, int32_t*, cudaStream_t)
 zmoe_status launch_encode_chunks(const zmoe_enc_chunk*, int, int, uint32_t*, cudaStream_t);
 zmoe_status launch_router(const zmoe_router_args*, cudaStream_t);
 zmoe_status launch_permute(const zmoe_permute_args*, cudaStream_t);
+int permute_launches(const zmoe_permute_args*);
 zmoe_status launch_combine(const zmoe_combine_args*, cudaStream_t);
 zmoe_status launch_permute_grad(const zmoe_permute_grad_args*, cudaStream_t);
 zmoe_status launch_combine_grad(const zmoe_combine_grad_args*, cudaStream_t);
@@ -69,6 +70,8 @@ zmoe_status zmoe_lz4_encode_chunks(const zmoe_enc_chunk* chunks, int n_chunks, i
 zmoe_status zmoe_router(const zmoe_router_args* a, zmoe_stream_t stream) {
   return zmoe::launch_router(a, reinterpret_cast<cudaStream_t>(stream));
 }
+
+int zmoe_permute_launches(const zmoe_permute_args* a) { return a && a->E >= 1 && a->k >= 1 ? zmoe::permute_launches(a) : 0; }
 
 zmoe_status zmoe_permute(const zmoe_permute_args* a, zmoe_stream_t stream) {
   return zmoe::launch_permute(a, reinterpret_cast<cudaStream_t>(stream));

@@ -27,6 +27,7 @@ namespace zmoe {
 zmoe_status launch_decode_chunks(const zmoe_chunk*, int, int32_t*, cudaStream_t);
 zmoe_status launch_router(const zmoe_router_args*, cudaStream_t);
 zmoe_status launch_permute(const zmoe_permute_args*, cudaStream_t);
+int permute_launches(const zmoe_permute_args*);
 zmoe_status launch_combine(const zmoe_combine_args*, cudaStream_t);
 
 namespace {
@@ -811,7 +812,7 @@ zmoe_status Layer::forward(const uint16_t* x, int T, uint16_t* out, cudaStream_t
   pa.seq_len = cfg.seq_len > 0 ? cfg.seq_len : T;
   pa.counts = counts; pa.offsets = offsets; pa.row_of = row_of; pa.token_of_row = tor; pa.xp = xp;
   if ((st = launch_permute(&pa, s)) != ZMOE_OK) return st;
-  stats.launches += 3;
+  stats.launches += permute_launches(&pa);
   ZMOE_CUDA_RET(cudaMemcpyAsync(counts_host, counts, sizeof(int32_t) * E, cudaMemcpyDeviceToHost, s));
   ZMOE_CUDA_RET(cudaEventRecord(counts_ready, s));
 

@@ -571,7 +571,42 @@ zmoe_status launch_sort(const SortArgs& a, cudaStream_t stream) {
   return launch_status("sort_kernel");
 }
 
+// The form a call takes, by its sizes alone.
+struct Plan {
+  enum Form { kNothing, kFused, kCluster, kWide, kRanked } form;
+  bool copy;                                           // a launch of its own for the rows
+  int per;                                             // kWide: steps per warp
+  int launches() const {
+    const int sort[] = {0, 1, 1, 3, 2};
+    return sort[form] + (copy ? 1 : 0);
+  }
+};
+Plan plan_of(const zmoe_permute_args* a) {
+  const int vec = a->H / 8;
+  Plan p{Plan::kNothing, false, 0};
+  if (a->T <= 0) return p;
+  p.copy = a->xp != nullptr && vec > 0;
+  p.form = Plan::kRanked;
+  if (a->capacity > 0 || a->E > kSortE || a->k > 32) return p;
+  p.form = Plan::kCluster;
+  const long long pairs = (long long)a->T * a->k;
+  if (p.copy && pairs <= kFusedPairs && (long long)a->T * vec < 1 << 30) {
+    p.form = Plan::kFused;
+    p.copy = false;
+    return p;
+  }
+  const int tp = 32 / a->k, steps = (int)(((long long)a->T + tp - 1) / tp);
+  const int per = (steps + kWideCtas * kSortWarps - 1) / (kWideCtas * kSortWarps);
+  if (pairs >= kWidePairs && kSortWarps * per * tp * a->k >= a->E) {
+    p.form = Plan::kWide;
+    p.per = per;
+  }
+  return p;
+}
+
 }  // namespace
+
+int permute_launches(const zmoe_permute_args* a) { return plan_of(a).launches(); }
 
 zmoe_status launch_permute(const zmoe_permute_args* a, cudaStream_t stream) {
   ZMOE_CHECK_ARG(a && a->topk_idx && a->counts && a->offsets && a->row_of && a->token_of_row,
@@ -588,11 +623,24 @@ zmoe_status launch_permute(const zmoe_permute_args* a, cudaStream_t stream) {
   }
   ZMOE_CHECK_ARG(a->T <= kMaxT && (long long)a->T * a->k < (1LL << 31), "permute: T=%d x k=%d pairs are too many", a->T, a->k);
   const int vec = a->H / 8;
+  const Plan plan = plan_of(a);
+  const size_t blocks = ((size_t)a->T * vec + kThreads - 1) / kThreads;
+  ZMOE_CHECK_ARG(!plan.copy || blocks < ((size_t)1 << 31), "permute: T=%d rows of H=%d are too many for one launch", a->T, a->H);
   zmoe_status st;
-  bool copies_tokens = false;
-  if (a->capacity <= 0 && a->E <= kSortE && a->k <= 32) {
-    SortArgs sa{a->topk_idx, a->T, a->k, a->E, 0, a->counts, a->offsets, a->row_of, a->token_of_row, 0};
-    if (a->xp && a->T * a->k <= kFusedPairs && vec > 0 && (long long)a->T * vec < 1 << 30) {
+  if (plan.form == Plan::kRanked) {
+    ZMOE_CUDA_RET(cudaMemsetAsync(a->row_of, 0xff, sizeof(int32_t) * (size_t)a->T * a->k, stream));
+    count_kernel<<<a->E, kThreads, 0, stream>>>(a->topk_idx, a->T, a->k, a->capacity, a->seq_len, a->counts);
+    st = launch_status("count_kernel");
+    if (st != ZMOE_OK) return st;
+    scatter_kernel<<<a->E, kThreads, 0, stream>>>(a->topk_idx, a->T, a->k, a->E, a->counts, a->offsets,
+                                                  a->row_of, a->token_of_row);
+    st = launch_status("scatter_kernel");
+  } else {
+    // behind a sort the copy of the rows writes token_of_row
+    const SortArgs sa{a->topk_idx, a->T, a->k, a->E, 0, a->counts, a->offsets, a->row_of,
+                      plan.copy ? nullptr : a->token_of_row, plan.per};
+    const int tp = 32 / a->k, steps = (a->T + tp - 1) / tp;
+    if (plan.form == Plan::kFused) {
       st = allow_smem<sort_gather_kernel>();
       if (st != ZMOE_OK) return st;
       const size_t smem = sort_smem(a->E) + sizeof(int32_t) * (size_t)a->T * a->k;
@@ -601,34 +649,16 @@ zmoe_status launch_permute(const zmoe_permute_args* a, cudaStream_t stream) {
       const int items = a->T * groups * vec;
       int per = (items / kNumSMs + 255) / 256 * 256;   // of a CTA at a time
       per = per < 256 ? 256 : per > kSortThreads ? kSortThreads : per;
-      int blocks = (items + per - 1) / per;
-      if (blocks > kNumSMs) blocks = kNumSMs;
-      sort_gather_kernel<<<blocks, kSortThreads, smem, stream>>>(sa, reinterpret_cast<const uint4*>(a->x), vec, groups, per,
-                                                                 reinterpret_cast<uint4*>(a->xp));
+      int ctas = (items + per - 1) / per;
+      if (ctas > kNumSMs) ctas = kNumSMs;
+      sort_gather_kernel<<<ctas, kSortThreads, smem, stream>>>(sa, reinterpret_cast<const uint4*>(a->x), vec, groups, per,
+                                                               reinterpret_cast<uint4*>(a->xp));
       return launch_status("sort_gather_kernel");
     }
-    if (a->xp && vec > 0) sa.token_of_row = nullptr;
-    const int tp = 32 / a->k, steps = (a->T + tp - 1) / tp;
-    const int per = (steps + kWideCtas * kSortWarps - 1) / (kWideCtas * kSortWarps);
-    if (a->T * a->k >= kWidePairs && kSortWarps * per * tp * a->k >= a->E) {
-      sa.wide = per;
-      st = launch_sort_wide(sa, (steps + kSortWarps * per - 1) / (kSortWarps * per), stream);
-    } else {
-      st = launch_sort(sa, stream);
-    }
-    copies_tokens = true;
-  } else {
-    ZMOE_CUDA_RET(cudaMemsetAsync(a->row_of, 0xff, sizeof(int32_t) * (size_t)a->T * a->k, stream));
-    count_kernel<<<a->E, kThreads, 0, stream>>>(a->topk_idx, a->T, a->k, a->capacity, a->seq_len, a->counts);
-    st = launch_status("count_kernel");
-    if (st != ZMOE_OK) return st;
-    scatter_kernel<<<a->E, kThreads, 0, stream>>>(a->topk_idx, a->T, a->k, a->E, a->counts, a->offsets,
-                                                  a->row_of, a->token_of_row);
-    st = launch_status("scatter_kernel");
+    st = plan.form == Plan::kWide ? launch_sort_wide(sa, (steps + kSortWarps * plan.per - 1) / (kSortWarps * plan.per), stream)
+                                  : launch_sort(sa, stream);
   }
-  if (st != ZMOE_OK || a->xp == nullptr || vec == 0) return st;
-  const size_t blocks = ((size_t)a->T * vec + kThreads - 1) / kThreads;
-  ZMOE_CHECK_ARG(blocks < ((size_t)1 << 31), "permute: T=%d rows of H=%d are too many for one launch", a->T, a->H);
+  if (st != ZMOE_OK || !plan.copy) return st;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3(kThreads);
@@ -640,7 +670,7 @@ zmoe_status launch_permute(const zmoe_permute_args* a, cudaStream_t stream) {
   cfg.numAttrs = 1;
   ZMOE_CUDA_RET(cudaLaunchKernelEx(&cfg, scatter_rows_kernel, reinterpret_cast<const uint4*>(a->x), a->T, vec, a->k,
                                    (const int32_t*)a->row_of, reinterpret_cast<uint4*>(a->xp), a->T * a->k,
-                                   copies_tokens ? a->token_of_row : (int32_t*)nullptr));
+                                   plan.form == Plan::kRanked ? (int32_t*)nullptr : a->token_of_row));
   return launch_status("scatter_rows_kernel");
 }
 

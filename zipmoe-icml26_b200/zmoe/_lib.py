@@ -119,6 +119,7 @@ SIGNATURES = {
     "zmoe_decode_chunks": (c_int, [c_void_p, c_int, c_void_p, c_void_p]),
     "zmoe_decode_scratch_bytes": (ctypes.c_uint64, [c_u32]),
     "zmoe_router": (c_int, [ctypes.POINTER(RouterArgs), c_void_p]),
+    "zmoe_permute_launches": (c_int, [ctypes.POINTER(PermuteArgs)]),
     "zmoe_permute": (c_int, [ctypes.POINTER(PermuteArgs), c_void_p]),
     "zmoe_expert_ffn": (c_int, [ctypes.POINTER(FfnArgs), c_void_p]),
     "zmoe_expert_ffn_noalloc": (c_int, [ctypes.POINTER(FfnArgs), c_void_p]),

@@ -273,6 +273,13 @@ def permute(topk_idx: torch.Tensor, x: Optional[torch.Tensor], E: int, capacity:
     return counts, offsets, row_of, tor, xp
 
 
+def permute_launches(T: int, k: int, E: int, H: int = 0, capacity: int = 0) -> int:
+    """Kernels that one permute launches, with rows of H to copy (0: without x)."""
+    xp = 16 if H else None                              # looked at for NULL alone
+    a = PermuteArgs(None, None, T, H, E, k, capacity, T, None, None, None, None, xp)
+    return lib.zmoe_permute_launches(ctypes.byref(a))
+
+
 def weight_table(mats: Sequence[Sequence[Optional[torch.Tensor]]], device=None) -> torch.Tensor:
     """Host array [G*3] of device weight pointers from per-group (w0, w1, w2)
     (the FFN builds one TMA descriptor per matrix on the host)."""
