@@ -251,7 +251,8 @@ zmoe_status zmoe_combine(const zmoe_combine_args* a, zmoe_stream_t stream);
  * products are fp32 in a fixed order, each output is rounded once; no atomics,
  * so results repeat bit for bit.  H must be a multiple of 8, every row pointer
  * 16-byte aligned.  row_of is zmoe_permute's; entries outside [0, rows) are
- * slots without a row.
+ * slots without a row.  Here and below an output overlaps no operand and no other
+ * output, unless it says so; calls whose memory overlaps are refused.
  * ------------------------------------------------------------------------ */
 /* dx[t] = base[t] + sum_j dxp[row_of[t, j]] (no base term when NULL).  base may
  * be dx itself. */
@@ -270,7 +271,9 @@ zmoe_status zmoe_permute_grad(const zmoe_permute_grad_args* a, zmoe_stream_t str
  *   dy_shared[t] = g[t] dout[t]              dshared_gate[t] = <dout[t], y_shared[t]>
  * mode SWITCH: a token without a row has dx[t] = w[t, 0] dout[t] and dtopk_w =
  * <dout[t], x[t]>; dx[t] = 0 for the others.  Slots without a row otherwise
- * have dtopk_w = 0.  Rows of dy that no slot names are left as they were. */
+ * have dtopk_w = 0.  Rows of dy that no slot names are left as they were.  An
+ * output may be its own operand: dy y, dtopk_w topk_w, dy_shared y_shared,
+ * dshared_gate shared_gate, dx x. */
 typedef struct zmoe_combine_grad_args {
   const uint16_t* dout;       /* [T, H] BF16 */
   const uint16_t* y;          /* [rows, H] BF16 expert rows */
@@ -338,7 +341,8 @@ zmoe_status zmoe_lora(const zmoe_lora_args* a, zmoe_stream_t stream);
  *   dx[t] = base[t] + v A      dA_g = sum of v^T x over the rows of g      dB_g = scale * sum of dy^T u
  * (the gradient of zmoe_lora's base is dy itself).  Tokens without adapter:
  * dx = base.  da and db are written whole: zeros for adapters without rows and
- * from the rank on.  dx, or da and db, may be NULL; dx is neither dy nor x.
+ * from the rank on.  dx, or da and db, may be NULL; with da and db, dx is neither
+ * dy nor x.
  * Sizes as for zmoe_lora, and G <= 65535. */
 typedef struct zmoe_lora_grad_args {
   const uint16_t* dy;         /* [T, N] BF16 */

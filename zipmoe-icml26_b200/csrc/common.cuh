@@ -43,6 +43,34 @@ inline zmoe_status launch_status(const char* what) {
   return ZMOE_OK;
 }
 
+// A piece of memory that a call reads or writes.  `twin`: the operand whose place a
+// written piece may take, whole.
+struct Span {
+  const char* what;
+  const void* p;
+  size_t bytes;
+  const char* twin = "";
+};
+// Whether each written piece lies apart from all read ones and from the other written
+// ones (NULL is no piece); else *a and *b name two that do not.
+template <int W, int R>
+bool apart(const Span (&written)[W], const Span (&read)[R], const char** a, const char** b) {
+  auto meet = [&](const Span& w, const Span& o) {
+    if (!w.p || !o.p || (w.p == o.p && w.bytes == o.bytes && !strcmp(w.twin, o.what))) return false;
+    const char *p = static_cast<const char*>(w.p), *q = static_cast<const char*>(o.p);
+    *a = w.what;
+    *b = o.what;
+    return p < q + o.bytes && q < p + w.bytes;
+  };
+  for (int i = 0; i < W; ++i) {
+    for (int j = 0; j < R; ++j)
+      if (meet(written[i], read[j])) return false;
+    for (int j = 0; j < i; ++j)
+      if (meet(written[i], written[j])) return false;
+  }
+  return true;
+}
+
 constexpr int kNumSMs = 148;
 
 // Lets a kernel use all of an SM's shared memory (227 KB, of which up to 1 KB

@@ -252,6 +252,15 @@ zmoe_status launch_lora(const zmoe_lora_args* a, cudaStream_t stream) {
                      aligned16(a->u) && aligned16(a->scratch), "lora: rows must be 16-byte aligned");
   ZMOE_CHECK_ARG(a->H <= kMaxCols && a->N <= kMaxCols, "lora: H=%d or N=%d above %d", a->H, a->N, kMaxCols);
   ZMOE_CHECK_ARG(a->T <= kMaxT, "lora: T=%d above %d", a->T, kMaxT);
+  {
+    const size_t T = a->T, H = a->H, N = a->N, G = a->G, R = a->R;
+    const Span w[] = {{"out", a->out, 2 * T * N, "base"}, {"u", a->u, 4 * T * R}, {"scratch", a->scratch, 4 * T * R}};
+    const Span r[] = {{"x", a->x, 2 * T * H}, {"base", a->base, 2 * T * N}, {"a", a->a, 2 * G * R * H}, {"b", a->b, 2 * G * N * R},
+                      {"scale", a->scale, 4 * G}, {"rank", a->rank, 4 * G}, {"offsets", a->offsets, 4 * (G + 1)},
+                      {"token_of_row", a->token_of_row, 4 * T}};
+    const char *p, *q;
+    ZMOE_CHECK_ARG(apart(w, r, &p, &q), "lora: %s must not overlap %s", p, q);
+  }
   // Few rows for each adapter: the rows kernel; else tiles of 128.  Measured (us, rows
   // against tiles, 2048 in and out): 512 rows 11.1 and 11.2 with one adapter of rank
   // 64, 12.5 and 24.7 with 128 of rank 16; 1024 rows 17.2 and 13.9, 11.7 and 12.9 at
@@ -301,6 +310,20 @@ zmoe_status launch_lora_grad(const zmoe_lora_grad_args* a, cudaStream_t stream) 
                  "lora_grad: rows must be 16-byte aligned");
   // dA and dB read dy and x after dx is written
   ZMOE_CHECK_ARG(!a->dx || !a->da || (a->dx != a->dy && a->dx != a->x), "lora_grad: dx must not be dy or x");
+  {
+    // without dA and dB, x and u are not read, and dx may be dy: its rows are written
+    // after the first product has read them all
+    const size_t T = a->T, H = a->H, N = a->N, G = a->G, R = a->R;
+    const void* base = a->dx ? a->base : nullptr;
+    const Span w[] = {{"dx", a->dx, 2 * T * H, base == a->dx ? "base" : a->da ? "" : "dy"}, {"da", a->da, 2 * G * R * H},
+                      {"db", a->db, 2 * G * N * R}, {"scratch", a->scratch, 4 * T * R}};
+    const Span r[] = {{"dy", a->dy, 2 * T * N}, {"x", a->da ? a->x : nullptr, 2 * T * H}, {"u", a->da ? a->u : nullptr, 4 * T * R},
+                      {"a", a->a, 2 * G * R * H}, {"b", a->b, 2 * G * N * R}, {"scale", a->scale, 4 * G},
+                      {"rank", a->rank, 4 * G}, {"offsets", a->offsets, 4 * (G + 1)},
+                      {"token_of_row", a->token_of_row, 4 * T}, {"base", base, 2 * T * H}};
+    const char *p, *q;
+    ZMOE_CHECK_ARG(apart(w, r, &p, &q), "lora_grad: %s must not overlap %s", p, q);
+  }
   return launch_grad_tiles(a, stream);
 }
 

@@ -165,6 +165,13 @@ zmoe_status launch_permute_grad(const zmoe_permute_grad_args* a, cudaStream_t st
   ZMOE_CHECK_ARG(a->H > 0 && a->H % 8 == 0, "permute_grad: H=%d must be a positive multiple of 8", a->H);
   ZMOE_CHECK_ARG(aligned16(a->dxp) && aligned16(a->base) && aligned16(a->dx),
                  "permute_grad: rows must be 16-byte aligned");
+  {
+    const size_t row = 2 * (size_t)a->H, T = a->T;
+    const Span w[] = {{"dx", a->dx, T * row, "base"}};
+    const Span r[] = {{"dxp", a->dxp, a->rows * row}, {"row_of", a->row_of, 4 * T * a->k}, {"base", a->base, T * row}};
+    const char *p, *q;
+    ZMOE_CHECK_ARG(apart(w, r, &p, &q), "permute_grad: %s must not overlap %s", p, q);
+  }
   const int vec = a->H / 8;
   const size_t blocks = ((size_t)a->T * vec + kThreads - 1) / kThreads;
   ZMOE_CHECK_ARG(blocks < ((size_t)1 << 31), "permute_grad: T=%d rows of H=%d are too many for one launch", a->T, a->H);
@@ -197,6 +204,19 @@ zmoe_status launch_combine_grad(const zmoe_combine_grad_args* a, cudaStream_t st
   ZMOE_CHECK_ARG(aligned16(a->dout) && aligned16(a->y) && aligned16(a->dy) && aligned16(a->y_shared) &&
                      aligned16(a->dy_shared) && aligned16(a->x) && aligned16(a->dx),
                  "combine_grad: rows must be 16-byte aligned");
+  {
+    // A warp reads a row's elements before it writes them, so an output may take the
+    // place of its own operand; dout is read by several.
+    const size_t row = 2 * (size_t)a->H, T = a->T;
+    const Span w[] = {{"dy", a->dy, a->rows * row, "y"}, {"dtopk_w", a->dtopk_w, 4 * T * a->k, "topk_w"},
+                      {"dy_shared", a->dy_shared, T * row, "y_shared"}, {"dshared_gate", a->dshared_gate, 4 * T, "shared_gate"},
+                      {"dx", a->dx, T * row, "x"}};
+    const Span r[] = {{"dout", a->dout, T * row}, {"y", a->y, a->rows * row}, {"y_shared", a->y_shared, T * row},
+                      {"shared_gate", a->shared_gate, 4 * T}, {"row_of", a->row_of, 4 * T * a->k},
+                      {"topk_w", a->topk_w, 4 * T * a->k}, {"x", a->x, T * row}};
+    const char *p, *q;
+    ZMOE_CHECK_ARG(apart(w, r, &p, &q), "combine_grad: %s must not overlap %s", p, q);
+  }
   const int slots = a->k + (a->dy_shared || a->dshared_gate ? 1 : 0);
   const size_t blocks = ((size_t)a->T * slots + kThreads / 32 - 1) / (kThreads / 32);
   ZMOE_CHECK_ARG(blocks < ((size_t)1 << 31), "combine_grad: T=%d x k=%d is too many for one launch", a->T, a->k);

@@ -679,6 +679,10 @@ zmoe_status launch_lora_plan(const int32_t* adapter, int T, int G, int32_t* offs
   ZMOE_CHECK_ARG(G >= 1 && G < kSortE, "lora_plan: G=%d outside [1, %d]", G, kSortE - 1);
   ZMOE_CHECK_ARG(T >= 0 && offsets && (T == 0 || (adapter && token_of_row)), "lora_plan: null pointer or negative T");
   ZMOE_CHECK_ARG(T <= kMaxT, "lora_plan: T=%d above %d", T, kMaxT);
+  const Span w[] = {{"offsets", offsets, 4 * ((size_t)G + 1)}, {"token_of_row", T ? token_of_row : nullptr, 4 * (size_t)T}};
+  const Span r[] = {{"adapter", T ? adapter : nullptr, 4 * (size_t)T}};
+  const char *p, *q;
+  ZMOE_CHECK_ARG(apart(w, r, &p, &q), "lora_plan: %s must not overlap %s", p, q);
   if (T == 0) {
     ZMOE_CUDA_RET(cudaMemsetAsync(offsets, 0, sizeof(int32_t) * (size_t)(G + 1), stream));
     return ZMOE_OK;
