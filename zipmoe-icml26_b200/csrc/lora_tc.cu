@@ -820,7 +820,8 @@ struct DwArgs {
 // of 2047 rows.)
 // kWide: R <= 32, the terms lie side by side as the columns of one product (3 R), so that
 // an MMA reads the 128 columns of x or dy once for all of them; else a term has RB blocks
-// of 64 columns (R <= 64 RB), and the terms' products are added one by one.
+// of 64 columns (R <= 64 RB), and the second and third term's products share a sum.
+// Either way the first term's sum is cut to fp32 once per MMA, not once per term.
 template <int RB, bool kWide>
 struct Dw {
   static constexpr int kRows = 32, kCols = 2 * kTile;
@@ -830,7 +831,7 @@ struct Dw {
   static constexpr int kPerSM = RB == 1 ? 2 : 1;
   static constexpr int kStages = kWide ? 4 : RB == 1 ? 3 : 5;   // 96 / 84 / 200 KB
   static constexpr int kDepth = kWide ? 4 : 3;         // steps of the factor in registers
-  static constexpr uint32_t kTileCols = kWide ? 96 : RB * 64;   // of TMEM, for 128 columns of x or dy
+  static constexpr uint32_t kTileCols = kWide ? 96 : RB * 128;  // of TMEM, for 128 columns of x or dy
   static constexpr uint32_t kTmemCols = kWide ? 256 : 2 * kTileCols;
   static constexpr int kSmem = 1024 + kStages * kStageBytes;
 };
@@ -930,7 +931,7 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB, kWide>::kPerSM) lora_dw_ker
             const uint64_t da = dx0 + off + kk * (2048 >> 4) + n * (2 * D::kBlock >> 4);
 #pragma unroll
             for (int i = kWide ? 0 : 2; i >= 0; --i)
-              mma_ss(tmem + n * D::kTileCols, da, dw + i * (RB * D::kBlock >> 4), id, (!kWide && i != 2) || (s | kk) != 0, go);
+              mma_ss(tmem + n * D::kTileCols + (i ? RB * 64 : 0), da, dw + i * (RB * D::kBlock >> 4), id, i == 1 || (s | kk) != 0, go);
           }
         }
         commit_at(used_a + 8 * at.slot, go);
@@ -1056,15 +1057,16 @@ __global__ void __launch_bounds__(kDwThreads, Dw<RB, kWide>::kPerSM) lora_dw_ker
       float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       if (ns > 0) {
         const uint32_t at = tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(t * D::kTileCols + c8);
-        if (kWide) {
-          uint32_t w[3][8];
+        constexpr int kSums = kWide ? 3 : 2;
+        uint32_t w[kSums][8];
 #pragma unroll
-          for (int q = 0; q < 3; ++q) tmem_ld8(at + q * rp, w[q]);
-          tmem_wait_ld();
+        for (int q = 0; q < kSums; ++q) tmem_ld8(at + q * (kWide ? rp : RB * 64), w[q]);
+        tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(w[0][e]) + (__uint_as_float(w[1][e]) + __uint_as_float(w[2][e]));
-        } else {
-          tmem_ld8(at, v);
+        for (int e = 0; e < 8; ++e) {
+          v[e] = __uint_as_float(w[kSums - 1][e]);     // the small sums first
+#pragma unroll
+          for (int q = kSums - 2; q >= 0; --q) v[e] += __uint_as_float(w[q][e]);
         }
       }
       if (csize > 1) {
