@@ -135,14 +135,6 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&f)[8]) {
-  uint32_t r[8];
-  tmem_ld8(taddr, r);
-  tmem_wait_ld();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(r[i]);
-}
-
 __device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint4& v) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(v.x), "r"(v.y), "r"(v.z),
                "r"(v.w)
@@ -367,7 +359,7 @@ template <int DIR, int RB>
 __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora_shrink_kernel(const TileArgs a) {
   using L = Shrink<RB>;
   constexpr int kStages = L::kStages, kTurn = L::kGroups, kMmaWarp = kTurn * kLoadWarps;
-  constexpr uint32_t kTmemCols = RB * 64;
+  constexpr uint32_t kSum = RB * 64, kTmemCols = 2 * kSum;   // two sums, of half the steps each
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[kStages], used[kStages], sums, last;
   __shared__ uint32_t tmem_slot;
@@ -467,7 +459,7 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
       fence_async();
       const uint32_t off = at.slot * (L::kStageBytes >> 4);
 #pragma unroll
-      for (int kk = 0; kk < kStep / 16; ++kk) mma_ss(tmem, dx0 + off + 2 * kk, dw0 + off + kPer * kk, id, (s | kk) != 0, go);
+      for (int kk = 0; kk < kStep / 16; ++kk) mma_ss(tmem + (kk & 1) * kSum, dx0 + off + 2 * kk, dw0 + off + kPer * kk, id, (s | kk >> 1) != 0, go);
       commit_at(used_a + 8 * at.slot, go);
       at.next();
     }
@@ -498,6 +490,15 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
     sp[0] = make_float4(f[0], f[1], f[2], f[3]);
     sp[1] = make_float4(f[4], f[5], f[6], f[7]);
   };
+  auto sums_of = [&](int i, float (&f)[8]) {
+    const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(8 * i);
+    uint32_t v[2][8];                                  // a tensor-core sum is cut, not rounded, at every MMA
+    tmem_ld8(at, v[0]);
+    tmem_ld8(at + kSum, v[1]);
+    tmem_wait_ld();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(v[0][e]) + __uint_as_float(v[1][e]);
+  };
   const int first = csize == 1 ? half : rank + csize * half, stride = 2 * csize;
   if (warp < kMmaWarp) wait_bar(smem_u32(&sums), 0, guard);   // every MMA has read the ring
   tc_fence_after();
@@ -505,14 +506,14 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
     if (warp < kMmaWarp)
       for (int i = first; i < n8; i += stride) {
         float f[8];
-        tmem_ld8(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(8 * i), f);
+        sums_of(i, f);
         write(i, f);
       }
   } else {
     if (warp < kMmaWarp)
       for (int i = half; i < n8; i += 2) {
         float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (nk > 0) tmem_ld8(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(8 * i), f);
+        if (nk > 0) sums_of(i, f);
         part[2 * i * kTile + m] = make_float4(f[0], f[1], f[2], f[3]);
         part[(2 * i + 1) * kTile + m] = make_float4(f[4], f[5], f[6], f[7]);
       }
