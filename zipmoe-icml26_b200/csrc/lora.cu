@@ -80,6 +80,7 @@ lora_rows_kernel(const zmoe_lora_args a) {
   const int hs = slice8(H, csize), h0 = min(H, rank * hs), h1 = min(H, h0 + hs);
   const int ns = slice8(N, csize), n0 = min(N, rank * ns), n1 = min(N, n0 + ns);
   const int tok = row < nm ? token_of(a.token_of_row, un.row0 + row, a.T) : -1;   // of this lane's column
+  const unsigned named = __ballot_sync(kFull, tok >= 0);   // bit 4 m: row m has a token
   int rk = 0;
   float scale = 1.0f;
   if (g < a.G) {
@@ -183,7 +184,7 @@ lora_rows_kernel(const zmoe_lora_args a) {
 #pragma unroll
     for (int c = 0; c < kCluster; ++c) s += p[c];
     const int m = i / R, r = i - m * R;
-    if (r >= rk || token_of(a.token_of_row, un.row0 + m, a.T) < 0) s = 0.0f;   // a row of no token has u = 0
+    if (r >= rk || !(named >> (4 * m) & 1)) s = 0.0f;   // a row of no token has u = 0
     if (rank == 0 && a.u) a.u[(size_t)un.row0 * R + i] = s;
     s *= scale;
     uint32_t t[3];
@@ -262,9 +263,9 @@ zmoe_status launch_lora(const zmoe_lora_args* a, cudaStream_t stream) {
     ZMOE_CHECK_ARG(apart(w, r, &p, &q), "lora: %s must not overlap %s", p, q);
   }
   // Few rows for each adapter: the rows kernel; else tiles of 128.  Measured (us, rows
-  // against tiles, 2048 in and out): 512 rows 11.1 and 11.2 with one adapter of rank
-  // 64, 12.5 and 24.7 with 128 of rank 16; 1024 rows 17.2 and 13.9, 11.7 and 12.9 at
-  // rank 16, 24.5 and 29.1 with 128 of rank 64; 2048 rows 29.4 and 16.4.
+  // against tiles, 2048 in and out): 512 rows 10.0 and 11.9 with one adapter of rank
+  // 64, 13.7 and 39 with 128 of rank 16; 1024 rows 14.9 and 14.3, 10.8 and 12.0 at
+  // rank 16, 28.7 and 51 with 128 of rank 64; 2048 rows 26.1 and 16.8.
   if (a->T > 2 * ZMOE_LORA_ROWS || (a->T > ZMOE_LORA_ROWS && a->R > 32 && a->G < 32)) return launch_tiles(a, stream);
   // as many CTAs per unit as fit the SMs together, two on each
   const int about = (a->T + kRows - 1) / kRows + (a->T < a->G ? a->T : a->G) / 2;

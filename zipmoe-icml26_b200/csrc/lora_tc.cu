@@ -14,7 +14,7 @@
 //                       the contraction, one tile of 256 columns of x or dy per
 //                       cluster, whose CTAs share the rows.
 // (A single kernel for shrink and expand, with u kept in TMEM, measured slower:
-// 31.5 against 29 us for 8191 rows of 2048 in and out at rank 64, 25 against 17 us
+// 31.5 against 28 us for 8191 rows of 2048 in and out at rank 64, 25 against 17 us
 // for 2047 rows of 2048 in and 5632 out at rank 16: tiles of whole rows leave SMs
 // without work.)
 //
@@ -554,23 +554,28 @@ __global__ void __launch_bounds__(Shrink<RB>::kThreads, Shrink<RB>::kPerSM) lora
 // ---------------------------------------------------------------------------
 // second product
 // ---------------------------------------------------------------------------
-template <int RB>
+// kDirect (R <= 32): a lane loads its row of the operand itself; else the rows come
+// through shared memory, as a lane's 16 bytes are half a sector of a row of its own
+// (us, direct and through shared memory: 8191 rows at rank 64 30.8 and 28.3, at rank 16
+// 24.6 and 25.4; the gradient of 16380 rows at rank 32 79.6 and 82.2).
+template <int RB, bool kDirect>
 struct Expand {
   static constexpr uint32_t kStageBytes = kXBytes + RB * 8192;
   static constexpr int kPerSM = RB == 1 ? 2 : 1;
-  static constexpr int kStages = RB == 1 ? 4 : 6;      // 96 KB / 192 KB
+  static constexpr int kStages = kDirect || RB == 2 ? 4 : 3;   // 96 / 72 / 128 KB
+  static constexpr uint32_t kRowBytes = kDirect ? 0 : RB * 256;   // a row of the operand in fp32, behind the ring: 32 / 64 KB
   // TMEM: outputs of 64 columns, then the operand's terms, two BF16 a column
   static constexpr int kOuts = RB == 1 ? 2 : 4;
   static constexpr uint32_t kOperand = 64 * kOuts, kTerm = 32 * RB;
   static constexpr uint32_t kTmemCols = RB == 1 ? 256 : 512;
   static constexpr int kDrainWarps = 8;                // two groups, taking steps in turn
   static constexpr int kThreads = 32 * (kDrainWarps + 1 + kLoadWarps);
-  static constexpr int kSmem = 1024 + kStages * kStageBytes;
+  static constexpr int kSmem = 1024 + kStages * kStageBytes + kTile * kRowBytes;
 };
 
-template <int DIR, int RB>
-__global__ void __launch_bounds__(Expand<RB>::kThreads, Expand<RB>::kPerSM) lora_expand_kernel(const TileArgs a) {
-  using L = Expand<RB>;
+template <int DIR, int RB, bool kDirect>
+__global__ void __launch_bounds__(Expand<RB, kDirect>::kThreads, Expand<RB, kDirect>::kPerSM) lora_expand_kernel(const TileArgs a) {
+  using L = Expand<RB, kDirect>;
   constexpr int kStages = L::kStages, kDrainWarps = L::kDrainWarps, kOuts = L::kOuts;
   constexpr uint32_t kTmemCols = L::kTmemCols;
   extern __shared__ uint8_t smem_raw[];
@@ -717,21 +722,38 @@ __global__ void __launch_bounds__(Expand<RB>::kThreads, Expand<RB>::kPerSM) lora
     finish_mmas(&last, go, a.limit);
   } else {
     // ------------------------------------------------------------------ operand
-    // The first product's sums of this lane's row, every other eight columns, in three
-    // BF16 terms.  They were written beside this launch's beginning: loads past L1.
+    // The first product's sums into TMEM in three BF16 terms, a row a lane, every other
+    // eight columns.  They were written beside this launch's beginning: loads past L1.
     const int m = q * 32 + lane;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     {
       const int c_end = rp / 8, c_in = min(rp, R) / 8; // zeros between them
-      const float4* p = reinterpret_cast<const float4*>(a.second + (size_t)(un.row0 + min(m, un.rows - 1)) * R);
+      const uint8_t* staged = smem + kStages * L::kStageBytes + m * L::kRowBytes;
+      if (!kDirect) {
+        const uint32_t op = ring + kStages * L::kStageBytes;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int row = (tid >> 3) + 32 * j;
+          const float* p = a.second + (size_t)(un.row0 + min(row, un.rows - 1)) * R;
+#pragma unroll
+          for (int e = 0; e < 2 * RB; ++e) {
+            const int c = (tid & 7) + 8 * e;           // of four columns, 128-byte swizzled
+            if (c < 2 * c_in) cp16(op + row * L::kRowBytes + 16u * (uint32_t)(c ^ (row & 7)), p + 4 * c);
+          }
+        }
+        cp_wait_all();
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * L::kDrainWarps) : "memory");
+      }
+      const float4* row = reinterpret_cast<const float4*>(a.second + (size_t)(un.row0 + min(m, un.rows - 1)) * R);
       float4 v[4 * RB][2];
 #pragma unroll
       for (int e = 0; e < 4 * RB; ++e) {
         const int c = half + 2 * e;
         v[e][0] = v[e][1] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (c < c_in) {
-          v[e][0] = __ldcg(p + 2 * c);
-          v[e][1] = __ldcg(p + 2 * c + 1);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            v[e][h] = kDirect ? __ldcg(row + 2 * c + h) : *reinterpret_cast<const float4*>(staged + 16 * ((2 * c + h) ^ (m & 7)));
         }
       }
 #pragma unroll
@@ -1155,14 +1177,14 @@ int share(long long units, int steps, int places, int fixed, int fixed_shared, i
   return best;
 }
 
-template <int DIR, int RB>
+template <int DIR, int RB, bool kDirect>
 zmoe_status launch_tiles(TileArgs a, cudaStream_t stream) {
   const long long units = a.T / kTile + (a.T < a.G + 2 ? a.T : a.G + 2);       // at most
   const int tiles = (a.T + kTile - 1) / kTile + (a.T < a.G ? a.T : a.G) / 2;   // about
   using S = Shrink<RB>;
-  using E = Expand<RB>;
+  using E = Expand<RB, kDirect>;
   zmoe_status st = allow_smem<lora_shrink_kernel<DIR, RB>>();
-  if (st == ZMOE_OK) st = allow_smem<lora_expand_kernel<DIR, RB>>();
+  if (st == ZMOE_OK) st = allow_smem<lora_expand_kernel<DIR, RB, kDirect>>();
   if (st != ZMOE_OK) return st;
   const int c = share(tiles, (a.K1 + kStep - 1) / kStep, kNumSMs * S::kPerSM, 2, 8, 8, true);
   const int steps2 = (a.K2 + kStep - 1) / kStep;
@@ -1182,8 +1204,15 @@ zmoe_status launch_tiles(TileArgs a, cudaStream_t stream) {
   st = launch(lora_shrink_kernel<DIR, RB>, dim3((unsigned)(units * c)), S::kThreads, c, false, S::kSmem, stream, a,
               "lora_shrink_kernel");
   if (st != ZMOE_OK || !a.out) return st;
-  return launch(lora_expand_kernel<DIR, RB>, dim3((unsigned)(units * a.parts)), E::kThreads, 1, true, E::kSmem, stream, a,
+  return launch(lora_expand_kernel<DIR, RB, kDirect>, dim3((unsigned)(units * a.parts)), E::kThreads, 1, true, E::kSmem, stream, a,
                 "lora_expand_kernel");
+}
+
+template <int DIR>
+zmoe_status launch_tiles(const TileArgs& a, cudaStream_t stream) {
+  return a.R <= 32   ? launch_tiles<DIR, 1, true>(a, stream)
+         : a.R <= 64 ? launch_tiles<DIR, 1, false>(a, stream)
+                     : launch_tiles<DIR, 2, false>(a, stream);
 }
 
 template <int RB, bool kWide>
@@ -1213,13 +1242,13 @@ zmoe_status launch_dw(const DwArgs& a, cudaStream_t stream) {
 zmoe_status launch_tiles(const zmoe_lora_args* p, cudaStream_t stream) {
   const TileArgs a{p->x, p->a, p->b, p->base, p->scale, p->rank, p->offsets, p->token_of_row, p->T, p->H, p->N, p->G,
                    p->R, p->out, p->u, p->scratch, 0, 1, tc::wait_limit(), tc::drop_loads()};
-  return p->R <= 64 ? launch_tiles<0, 1>(a, stream) : launch_tiles<0, 2>(a, stream);
+  return launch_tiles<0>(a, stream);
 }
 
 zmoe_status launch_grad_tiles(const zmoe_lora_grad_args* p, cudaStream_t stream) {
   const TileArgs a{p->dy, p->b, p->a, p->base, p->scale, p->rank, p->offsets, p->token_of_row, p->T, p->N, p->H, p->G,
                    p->R, p->dx, nullptr, p->scratch, p->da ? (long long)p->G * ((p->N + 2 * kTile - 1) / (2 * kTile)) : 0, 1, tc::wait_limit(), tc::drop_loads()};
-  zmoe_status st = p->R <= 64 ? launch_tiles<1, 1>(a, stream) : launch_tiles<1, 2>(a, stream);
+  zmoe_status st = launch_tiles<1>(a, stream);
   if (st != ZMOE_OK || !p->da) return st;
   const DwArgs d{{p->x, p->dy}, {p->scratch, p->u}, {p->da, p->db}, p->scale, p->rank, p->offsets, p->token_of_row,
                  {p->H, p->N}, p->T, p->G, p->R, tc::wait_limit(), tc::drop_loads()};
