@@ -58,7 +58,8 @@ __device__ __forceinline__ uint4 keep(uint4 v, int left) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// KB: 32-wide blocks of the rank (R <= 32 * KB).
+// KB: 32-wide blocks of the rank (R <= 32 * KB).  The fewer, the more tiles of B are in
+// flight beside s u (96 requests of rank 16 15.2 us with room for two blocks, 13.0 for one).
 template <int KB>
 __global__ void __launch_bounds__(kThreads, 2)
 lora_rows_kernel(const zmoe_lora_args a) {
@@ -264,7 +265,7 @@ zmoe_status launch_lora(const zmoe_lora_args* a, cudaStream_t stream) {
   }
   // Few rows for each adapter: the rows kernel; else tiles of 128.  Measured (us, rows
   // against tiles, 2048 in and out): 512 rows 10.0 and 11.9 with one adapter of rank
-  // 64, 13.7 and 39 with 128 of rank 16; 1024 rows 14.9 and 14.3, 10.8 and 12.0 at
+  // 64, 12.8 and 39 with 128 of rank 16; 1024 rows 14.9 and 14.3, 9.4 and 12.0 at
   // rank 16, 28.7 and 51 with 128 of rank 64; 2048 rows 26.1 and 16.8.
   if (a->T > 2 * ZMOE_LORA_ROWS || (a->T > ZMOE_LORA_ROWS && a->R > 32 && a->G < 32)) return launch_tiles(a, stream);
   // as many CTAs per unit as fit the SMs together, two on each
@@ -282,7 +283,7 @@ zmoe_status launch_lora(const zmoe_lora_args* a, cudaStream_t stream) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  ZMOE_CUDA_RET(cudaLaunchKernelEx(&cfg, a->R <= 64 ? lora_rows_kernel<2> : lora_rows_kernel<4>, *a));
+  ZMOE_CUDA_RET(cudaLaunchKernelEx(&cfg, a->R <= 32 ? lora_rows_kernel<1> : a->R <= 64 ? lora_rows_kernel<2> : lora_rows_kernel<4>, *a));
   return launch_status("lora_rows_kernel");
 }
 
