@@ -12,7 +12,9 @@
 //                       the shrink: it loads base and weights while that ends.
 //   lora_dw_kernel      dA^T = x^T v and dB = s dy^T u: the rows of an adapter as
 //                       the contraction, one tile of 256 columns of x or dy per
-//                       cluster, whose CTAs share the rows.
+//                       cluster, whose CTAs share the rows.  dB needs nothing of
+//                       the launches in front and runs beside them; dA waits for
+//                       them.
 // (A single kernel for shrink and expand, with u kept in TMEM, measured slower:
 // 31.5 against 28 us for 8191 rows of 2048 in and out at rank 64, 25 against 17 us
 // for 2047 rows of 2048 in and 5632 out at rank 16: tiles of whole rows leave SMs
@@ -25,7 +27,7 @@
 // memory, but moved the outputs four times as far from an fp32 product's as the order
 // of its sums does.)
 //
-// Warps have roles: some load, one issues the MMAs, some drain TMEM.  Operands
+// Warps have roles: some load, some split, one issues the MMAs, some drain TMEM.  Operands
 // come in by cp.async (rows are gathered by token, 16 bytes a lane) into
 // 128-byte-swizzled tiles of a ring, whose slots pass from role to role by
 // mbarriers, so that no step waits for the whole CTA.  Every column beyond an
